@@ -212,6 +212,139 @@ int lmx_sdpa_decode_noalloc(const void* q, const lmx_kv* kv, int T, int heads, f
                             void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged KV cache: many requests of unequal lengths in one batch.
+ *
+ * The cache is a pool of pages; a page holds page_size rows of every KV head.
+ * Row p of sequence s lies in page block_table[s][p / page_size], slot
+ * p % page_size.  The new tokens of all sequences are packed one after
+ * another: sequence s owns tokens q_start[s] .. q_start[s+1]-1, and its last
+ * token is at position kv_len[s]-1, so its i-th new token is at position
+ * kv_len[s] - (q_start[s+1] - q_start[s]) + i.  A sequence may have no new
+ * token.  The index arrays are read on the device when the call runs; a
+ * position below 0 (kv_len smaller than the new tokens) has no row: it is not
+ * appended, it is gathered and attended as zeros.  An entry of the table that
+ * names no page of the pool, and a position past table_stride pages (or past
+ * the rotation tables), sets the device error word to 0x44
+ * (lmx_device_error): its row is not written and reads as zeros.
+ * The reference keeps one contiguous cache per request (src/common/
+ * kv_cache.cpp:34-142, :243-377) and has no paged form.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  int pages, page_size;     /* page_size 16, 32, 64, 128 or 256               */
+  int kv_heads, head_dim;   /* head_dim 64 or 128                             */
+  int bits;                 /* 16 = bf16 rows, 8 or 4 = affine, group 64      */
+  int64_t page_stride;      /* rows from one page to the next (a row: one
+                             * head's values); 0 = kv_heads * page_size.  For
+                             * bits 8 / 4 a multiple of 16 and the same for the
+                             * packed, scale and bias arrays                  */
+  void* k;                  /* bits 16: bf16 [pages][kv_heads][page_size][head_dim] */
+  void* v;
+  uint32_t* k_packed;       /* bits 8 / 4: [pages][kv_heads][page_size][head_dim*bits/32];
+                             * k, v and the packed arrays 16-byte aligned     */
+  uint32_t* v_packed;
+  void* k_scales;           /* bits 8 / 4: bf16 [pages][kv_heads][page_size][head_dim/64],
+                             * 16-byte aligned                                */
+  void* k_biases;
+  void* v_scales;
+  void* v_biases;
+} lmx_paged_kv;
+
+typedef struct {
+  int seqs;                   /* sequences, at most 2048                        */
+  int tokens;                 /* packed rows: at least q_start[seqs]            */
+  int max_new;                /* at least the most new tokens of one sequence   */
+  const int32_t* q_start;     /* device [seqs+1], ascending, q_start[0] >= 0    */
+  const int32_t* kv_len;      /* device [seqs]: rows, the new tokens included   */
+  const int32_t* block_table; /* device [seqs][table_stride] page numbers       */
+  int table_stride;
+} lmx_paged_batch;
+
+/* Rotary positions.  A pair (a, b) of a head turns by position * frequency:
+ * a' = a*cos - b*sin, b' = b*cos + a*sin.  Pair i is (i, i + rot_dim/2), or
+ * (2i, 2i+1) when interleaved; values past rot_dim pass through (partial
+ * rotary).  cos / sin: device fp32 [positions][rot_dim/2], 16-byte aligned
+ * (lmx_rope_table fills them).  rot_dim is a multiple of 16, at most head_dim. */
+typedef struct {
+  const float* cos;
+  const float* sin;
+  int positions;
+  int rot_dim;
+  int interleaved;
+} lmx_rope;
+
+/* Frequencies theta^(-2i/rot_dim), stretched for a context longer than the
+ * trained one:
+ *   linear  f / factor;
+ *   llama3  the frequencies whose wavelength exceeds orig_positions/low are
+ *           divided by factor, those below orig_positions/high kept, a linear
+ *           ramp in orig_positions/wavelength in between (LlamaDynamicNTK-
+ *           ScalingRoPE, src/llm/models/llama.cpp:122-183);
+ *   yarn    a linear ramp over the pair index between the pairs that turn
+ *           `high` (beta_fast) and `low` (beta_slow) times within
+ *           orig_positions, rounded outwards to whole pairs, from f to
+ *           f / factor; cos and sin are multiplied by attn_factor
+ *           (0 = 0.1 ln(factor) + 1). */
+typedef enum { LMX_ROPE_PLAIN = 0, LMX_ROPE_LINEAR = 1, LMX_ROPE_LLAMA3 = 2, LMX_ROPE_YARN = 3 } lmx_rope_kind;
+typedef struct {
+  int kind;              /* lmx_rope_kind                                     */
+  double theta;
+  double factor;         /* >= 1; unused when plain                           */
+  double low, high;      /* llama3: low_freq_factor, high_freq_factor;
+                          * yarn: beta_slow, beta_fast                        */
+  double orig_positions; /* llama3, yarn                                      */
+  double attn_factor;    /* yarn                                              */
+} lmx_rope_scaling;
+/* Fill cos / sin [positions][rot_dim/2] (device fp32): angles in 64 bits,
+ * rounded once.  positions * rot_dim/2 < 2^31. */
+int lmx_rope_table(const lmx_rope_scaling* scaling, int positions, int rot_dim, float* cos_out, float* sin_out,
+                   void* stream);
+/* Rotate x [tokens][heads][head_dim] (bf16; token rows ldx values apart) by
+ * pos[t] into y (rows ldy apart); y may be x itself (same ldx).  inverse
+ * turns back: the gradient of the rotation, and its undoing.  head_dim a
+ * multiple of 16, at most 256.  A position outside [0, positions) leaves its
+ * row of y unwritten and sets the device error word to 0x44. */
+int lmx_rope_apply(const lmx_rope* rope, const void* x, int64_t ldx, const int32_t* pos, int tokens, int heads,
+                   int head_dim, int inverse, void* y, int64_t ldy, void* stream);
+
+/* Append the new tokens' K and V rows to the cache, the rotation of q and k
+ * on the way.  q [tokens][heads], k and v [tokens][kv_heads] heads of
+ * head_dim bf16 values, token rows ld values apart (the three parts of a
+ * fused projection's rows, or arrays of their own).  q and k are rotated at
+ * their token's position (rope NULL: left as they are), after a per-head
+ * RMSNorm when q_norm / k_norm (bf16 [head_dim], both or neither) are given;
+ * q goes to q_out (rows ldq_out apart; may be q itself with ldq_out = ld; q
+ * and q_out NULL: no queries), k and v to their pages.  The arithmetic is
+ * fp32, rounded once: to bf16, or by the 8 / 4-bit rule of lmx_kv_append,
+ * here on the fp32 values.  A token past q_start[seqs] is left alone; a
+ * token at a position below 0, or one that sets the error word, gets zeros
+ * in q_out.  Two sequences must not append to the same row. */
+int lmx_paged_append(const lmx_paged_kv* kv, const lmx_paged_batch* batch, const lmx_rope* rope, const void* q,
+                     const void* k, const void* v, int64_t ld, int heads, const void* q_norm, const void* k_norm,
+                     float eps, void* q_out, int64_t ldq_out, void* stream);
+/* Read rows back: k_out, v_out bf16 [tokens][kv_heads][head_dim] = the cached
+ * rows of the batch's tokens (for whole sequences: q_start = the running sum
+ * of kv_len), dequantized as bf16(scale*code + bias).  Either may be NULL. */
+int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* batch, void* k_out, void* v_out, void* stream);
+
+/* Attention of the new tokens over the cache (their own rows already
+ * appended): the token at position p of its sequence sees the cached rows
+ * max(0, p - window + 1) .. p (window 0: all up to p);
+ *   out = softmax(scale * q.k) v,   lse = ln sum exp(scale * q.k).
+ * q, out [tokens][heads][head_dim] bf16, token rows ldq / ldo values apart
+ * (out must not overlap q); lse fp32 [tokens][heads] or NULL.  heads is a
+ * multiple of kv_heads, at most 64 times it.  A row that sees nothing gives
+ * zeros and lse -infinity.  Rows of a page that no sequence
+ * position covers may hold anything (NaN included); every row below kv_len
+ * must hold finite values.  scratch: lmx_paged_attention_scratch_bytes of the
+ * same kv / batch / heads (0 and a message in lmx_last_error when the
+ * arguments are refused), 16-byte aligned, contents arbitrary; calls that
+ * overlap need scratch of their own. */
+size_t lmx_paged_attention_scratch_bytes(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads);
+int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch* batch, const void* q, int64_t ldq, int heads,
+                        float scale, int window, void* scratch, size_t scratch_bytes, void* out, int64_t ldo,
+                        float* lse, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Hybrid-model ops (configuration 4, Qwen3-Next-style decoder).
  *
  * Gated DeltaNet verify step: replaces Qwen3NextGatedDeltaNet's core between

@@ -96,7 +96,7 @@ LMX_DEV float warp_sum_xor(float v, int first, int last) {
 
 // Kernel launches issued by this library (eager launches and launches being
 // captured into a graph), for the host-side launch accounting.
-static std::atomic<long long> g_lmx_launches{0};
+inline std::atomic<long long> g_lmx_launches{0};
 static inline cudaError_t lmx_counted(cudaError_t e) {
   if (e == cudaSuccess) g_lmx_launches.fetch_add(1, std::memory_order_relaxed);
   return e;

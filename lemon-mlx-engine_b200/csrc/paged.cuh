@@ -1,0 +1,1001 @@
+// paged.cuh -- rotary positions, the paged KV cache (append with the rotation
+// and the quantizer on the way, read back) and attention of new tokens over
+// it, for few query rows per KV head (decode, short verify blocks).
+//
+// A page holds P rows of every KV head, [pages][Hk][P][D] (packed codes,
+// scales and biases in the same order), so one head's rows of a page are
+// contiguous.  Row p of sequence s is in page table[s][p / P], slot p % P.
+#pragma once
+#include "lmx_common.cuh"
+
+namespace lmx {
+
+static constexpr int kPagedMaxSeqs = 2048;
+static constexpr unsigned kPagedErr = 0x44u;  // position without a row
+
+struct PagedKv {
+  int pages, P, logP, Hk, bits;
+  int64_t pstride;            // rows from page to page
+  uint8_t *k, *v;             // bf16 rows or packed codes
+  bf16_t *ks, *kb, *vs, *vb;  // [..][D/64]
+};
+
+struct PagedBatch {
+  int seqs, tokens;
+  const int32_t *q_start, *kv_len, *table;
+  int table_stride;
+};
+
+LMX_DEV uint32_t pk_bf2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+LMX_DEV float ex2f(float x) {  // 2^x, hardware approximation (2 ulp)
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+LMX_DEV uint32_t bf2_fma3(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+LMX_DEV void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The sequence that owns packed token t: how many of q_start[1..seqs] are
+// <= t.  The warp probes 32 entries at a time; sequences without new tokens
+// are passed over because their entries repeat.
+LMX_DEV int paged_seq(const PagedBatch& b, int t, int lane) {
+  int lo = 0, n = b.seqs;
+  while (n > 0) {
+    const int step = (n + 31) / 32;
+    const int at = (lane + 1) * step;
+    const bool le = at <= n && __ldg(b.q_start + lo + at) <= t;
+    const int c = __popc(__ballot_sync(0xffffffffu, le));
+    lo += c * step;
+    n = min(step - 1, n - c * step);
+  }
+  return lo;
+}
+
+// Row index (in rows of one head's values) of position pos, head 0; -1 where
+// the table has no page of the pool for it.
+LMX_DEV int64_t paged_row(const PagedKv& kv, const PagedBatch& b, int seq, int pos) {
+  const int blk = pos >> kv.logP;
+  if (blk >= b.table_stride) return -1;
+  const int page = __ldg(b.table + (int64_t)seq * b.table_stride + blk);
+  if ((unsigned)page >= (unsigned)kv.pages) return -1;
+  return (int64_t)page * kv.pstride + (pos & (kv.P - 1));
+}
+
+// ---------------------------------------------------------------------------
+// Rotation tables: angle = position * frequency in 64 bits, cos and sin
+// rounded to fp32 once.  Set-up work, one thread per entry.
+// ---------------------------------------------------------------------------
+struct RopeFreqs {
+  double f[128];
+};
+__global__ void rope_table_kernel(RopeFreqs fr, double mul, int positions, int half, float* ct, float* st) {
+  grid_wait();
+  grid_launch_dependents();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= positions * half) return;
+  double s, c;
+  sincos((double)(i / half) * fr.f[i % half], &s, &c);
+  ct[i] = (float)(c * mul);
+  st[i] = (float)(s * mul);
+}
+
+LMX_DEV void bf8_unpack(const uint4 v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (e & 1) ? hi_bf(w[e >> 1]) : lo_bf(w[e >> 1]);
+}
+LMX_DEV uint4 bf8_pack(const float (&x)[8]) {
+  return make_uint4(pk_bf2(x[0], x[1]), pk_bf2(x[2], x[3]), pk_bf2(x[4], x[5]), pk_bf2(x[6], x[7]));
+}
+LMX_DEV void load8f(const float* p, float (&x)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+// ---------------------------------------------------------------------------
+// Rotation of [tokens][heads][dim].  Memory bound: each value is read and
+// written once.  A thread owns one 16-value unit of HPT consecutive heads of
+// a token -- 8 pairs (two 16-byte halves, rot/2 apart, or 16 neighbours when
+// interleaved), so both layouts move whole 16-byte vectors and the unit's
+// cos / sin stay in registers over the heads; units past rot are copied.
+// ---------------------------------------------------------------------------
+struct RopeArgs {
+  const float *ct, *st;
+  int positions, rot, inter, inverse;
+  const bf16_t* x;
+  int64_t ldx;
+  const int32_t* pos;
+  int tokens, heads, dim;
+  bf16_t* y;
+  int64_t ldy;
+  unsigned* err;
+};
+
+template <int HPT>
+__global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
+  grid_wait();
+  grid_launch_dependents();
+  const int units = a.dim / 16, hg = (a.heads + HPT - 1) / HPT;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.tokens * hg * units) return;
+  const int u = (int)(i % units), g = (int)(i / units % hg), t = (int)(i / units / hg);
+  const int p = __ldg(a.pos + t);
+  if ((unsigned)p >= (unsigned)a.positions) {
+    if (u == 0 && g == 0) atomicExch(a.err, kPagedErr);
+    return;
+  }
+  const bool turn = u * 16 < a.rot;
+  if (!turn && a.x == a.y) return;
+  const int d0 = turn && !a.inter ? 8 * u : 16 * u;               // first eight values
+  const int d1 = turn && !a.inter ? a.rot / 2 + 8 * u : d0 + 8;   // the other eight
+  const int h0 = g * HPT;
+  const bf16_t* x = a.x + (int64_t)t * a.ldx + (int64_t)h0 * a.dim;
+  bf16_t* y = a.y + (int64_t)t * a.ldy + (int64_t)h0 * a.dim;
+  uint4 v0[HPT], v1[HPT];
+#pragma unroll
+  for (int k = 0; k < HPT; ++k) {
+    if (h0 + k < a.heads) {
+      v0[k] = *reinterpret_cast<const uint4*>(x + k * a.dim + d0);
+      v1[k] = *reinterpret_cast<const uint4*>(x + k * a.dim + d1);
+    }
+  }
+  float c[8], s[8];
+  if (turn) {
+    load8f(a.ct + (int64_t)p * (a.rot / 2) + 8 * u, c);
+    load8f(a.st + (int64_t)p * (a.rot / 2) + 8 * u, s);
+    if (a.inverse)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = -s[e];
+  }
+#pragma unroll
+  for (int k = 0; k < HPT; ++k) {
+    if (h0 + k >= a.heads) break;
+    if (turn) {
+      float p0[8], p1[8];
+      bf8_unpack(v0[k], p0);
+      bf8_unpack(v1[k], p1);
+      float w[16];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { w[e] = p0[e]; w[8 + e] = p1[e]; }
+      float r0[8], r1[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float xa = a.inter ? w[2 * e] : w[e], xb = a.inter ? w[2 * e + 1] : w[8 + e];
+        const float ya = __fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e]));
+        const float yb = __fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e]));
+        if (a.inter) {
+          if (e < 4) { r0[2 * e] = ya; r0[2 * e + 1] = yb; }
+          else { r1[2 * e - 8] = ya; r1[2 * e - 7] = yb; }
+        } else {
+          r0[e] = ya;
+          r1[e] = yb;
+        }
+      }
+      v0[k] = bf8_pack(r0);
+      v1[k] = bf8_pack(r1);
+    }
+    *reinterpret_cast<uint4*>(y + k * a.dim + d0) = v0[k];
+    *reinterpret_cast<uint4*>(y + k * a.dim + d1) = v1[k];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Append.  A warp owns IT * (256 / D) consecutive heads (q heads, then k,
+// then v) of one token: D / 8 lanes per head, eight values per lane, so a
+// head's row moves as one contiguous run, the RMSNorm and the quantizer's
+// min / max are shuffles within the head's lanes, and the token's sequence,
+// page and cos / sin are looked up once per warp.  The rotation's partner
+// values (rot/2 apart) are rot/16 lanes away.  fp32 throughout, rounded
+// once; products and sums of the rotation are rounded separately.
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+  PagedKv kv;
+  PagedBatch b;
+  const float *ct, *st;  // null: no rotation
+  int positions, rot, inter;
+  const bf16_t *q, *k, *v;
+  int64_t ld;
+  int heads;             // q heads (0: none)
+  const bf16_t *qn, *kn;
+  float eps;
+  bf16_t* q_out;
+  int64_t ldqo;
+  unsigned* err;
+};
+
+template <int D, int IT>
+__global__ void __launch_bounds__(128) paged_append_kernel(AppendArgs a) {
+  constexpr int L = D / 8, HPW = 32 / L;
+  grid_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int nh = a.heads + 2 * a.kv.Hk, wpt = (nh + HPW * IT - 1) / (HPW * IT);
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (w >= (int64_t)a.b.tokens * wpt) return;
+  const int t = (int)(w / wpt), h0 = (int)(w % wpt) * HPW * IT;
+  const int i = lane % L, sub = lane / L;
+
+  // the rows do not depend on the token's place: load them first
+  uint4 raw[IT];
+  float x[8];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int h = h0 + it * HPW + sub;
+    raw[it] = make_uint4(0, 0, 0, 0);
+    if (h < nh) {
+      const bf16_t* src = h < a.heads ? a.q + (int64_t)h * D
+                          : h < a.heads + a.kv.Hk ? a.k + (int64_t)(h - a.heads) * D
+                                                  : a.v + (int64_t)(h - a.heads - a.kv.Hk) * D;
+      raw[it] = *reinterpret_cast<const uint4*>(src + (int64_t)t * a.ld + 8 * i);
+    }
+  }
+  const int seq = paged_seq(a.b, t, lane);
+  if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;  // padding
+  const int pos = __ldg(a.b.kv_len + seq) - (__ldg(a.b.q_start + seq + 1) - t);
+  int64_t row = -1;
+  if (pos >= 0) {
+    row = paged_row(a.kv, a.b, seq, pos);
+    if (a.ct && pos >= a.positions) row = -1;
+    if (row < 0 && lane == 0) atomicExch(a.err, kPagedErr);
+  }
+  const int RL = a.ct ? a.rot / 8 : 0;  // rotated lanes of a head
+  float c[8], s[8];
+  if (row >= 0 && i < RL) {
+    const int half = a.rot / 2;
+    if (a.inter) {  // four pairs per lane
+      const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.ct + (int64_t)pos * half + 4 * i));
+      const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.st + (int64_t)pos * half + 4 * i));
+      c[0] = c4.x; c[1] = c4.y; c[2] = c4.z; c[3] = c4.w;
+      s[0] = s4.x; s[1] = s4.y; s[2] = s4.z; s[3] = s4.w;
+    } else {
+      const int m = i < RL / 2 ? i : i - RL / 2;
+      load8f(a.ct + (int64_t)pos * half + 8 * m, c);
+      load8f(a.st + (int64_t)pos * half + 8 * m, s);
+    }
+  }
+  const int partner = i < RL ? (i < RL / 2 ? i + RL / 2 : i - RL / 2) : i;
+
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int h = h0 + it * HPW + sub;
+    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv.Hk, live = h < nh;
+    bf8_unpack(raw[it], x);
+    if (a.qn) {
+      float p = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p = __fmaf_rn(x[e], x[e], p);
+      p = warp_sum_xor(p, L / 2, 1);
+      if (is_q || is_k) {
+        const float f = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(p, (float)D), a.eps)));
+        float wn[8];
+        bf8_unpack(__ldg(reinterpret_cast<const uint4*>((is_q ? a.qn : a.kn) + 8 * i)), wn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], f), wn[e]);
+      }
+    }
+    if (RL && !a.inter) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], sub * L + partner);
+      if ((is_q || is_k) && i < RL && row >= 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[e] = i < RL / 2 ? __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]))
+                            : __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]));
+      }
+    } else if ((is_q || is_k) && i < RL && row >= 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float xa = x[2 * e], xb = x[2 * e + 1];
+        x[2 * e] = __fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e]));
+        x[2 * e + 1] = __fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e]));
+      }
+    }
+    if (is_q) {
+      if (row < 0)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+      *reinterpret_cast<uint4*>(a.q_out + (int64_t)t * a.ldqo + (int64_t)h * D + 8 * i) = bf8_pack(x);
+    }
+    const int hk = is_k ? h - a.heads : h - a.heads - a.kv.Hk;
+    const int64_t r = row + (int64_t)hk * a.kv.P;
+    if (a.kv.bits == 16) {
+      if (!is_q && live && row >= 0)
+        *reinterpret_cast<uint4*>((is_k ? a.kv.k : a.kv.v) + (r * D + 8 * i) * 2) = bf8_pack(x);
+      continue;
+    }
+    // min / max of a group of 64 = 8 lanes
+    float mn = x[0], mx = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) { mn = fminf(mn, x[e]); mx = fmaxf(mx, x[e]); }
+#pragma unroll
+    for (int off = 4; off >= 1; off >>= 1) {
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    }
+    if (is_q || !live || row < 0) continue;
+    const int nb = (1 << a.kv.bits) - 1;
+    bf16_t sb = f2bf(__fdiv_rn(__fsub_rn(mx, mn), (float)nb));
+    if (bf2f(sb) == 0.0f) sb = f2bf(1.0f);
+    const bf16_t bb = f2bf(mn);
+    const float sc = bf2f(sb), bi = bf2f(bb);
+    uint32_t q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int v = (int)rintf(__fdiv_rn(__fsub_rn(x[e], bi), sc));
+      q[e] = (uint32_t)(v < 0 ? 0 : (v > nb ? nb : v));
+    }
+    uint8_t* dst = is_k ? a.kv.k : a.kv.v;
+    if (a.kv.bits == 8) {
+      *reinterpret_cast<uint2*>(dst + r * D + 8 * i) =
+          make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+    } else {
+      uint32_t wd = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wd |= q[e] << (4 * e);
+      *reinterpret_cast<uint32_t*>(dst + r * (D / 2) + 4 * i) = wd;
+    }
+    if ((i & 7) == 0) {
+      (is_k ? a.kv.ks : a.kv.vs)[r * (D / 64) + (i >> 3)] = sb;
+      (is_k ? a.kv.kb : a.kv.vb)[r * (D / 64) + (i >> 3)] = bb;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Gather: the batch's rows back as bf16(fma(scale, code, bias)).  A warp owns
+// one token, its lanes the 8-value chunks of the K heads, then the V heads.
+// ---------------------------------------------------------------------------
+struct GatherArgs {
+  PagedKv kv;
+  PagedBatch b;
+  bf16_t *k, *v;
+  unsigned* err;
+};
+
+// eight codes of a row -> values
+LMX_DEV uint4 paged_dequant8(int bits, const uint8_t* base, const bf16_t* sc, const bf16_t* bi, int64_t r, int D, int c) {
+  const float s = bf2f(__ldg(sc + r * (D / 64) + c / 8)), b = bf2f(__ldg(bi + r * (D / 64) + c / 8));
+  float x[8];
+  if (bits == 8) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(base + r * D + 8 * c));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(s, (float)(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu), b);
+  } else {
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(base + r * (D / 2) + 4 * c));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(s, (float)((w >> (4 * e)) & 0xfu), b);
+  }
+  return bf8_pack(x);
+}
+
+template <int D>
+__global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
+  constexpr int L = D / 8;
+  grid_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (w >= a.b.tokens) return;
+  const int t = (int)w;
+  const int seq = paged_seq(a.b, t, lane);
+  if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;  // padding
+  const int pos = __ldg(a.b.kv_len + seq) - (__ldg(a.b.q_start + seq + 1) - t);
+  int64_t row = -1;
+  if (pos >= 0) {
+    row = paged_row(a.kv, a.b, seq, pos);
+    if (row < 0 && lane == 0) atomicExch(a.err, kPagedErr);
+  }
+  const int n = a.kv.Hk * L;
+#pragma unroll 4
+  for (int c = lane; c < 2 * n; c += 32) {
+    const bool is_k = c < n;
+    const int at = is_k ? c : c - n, h = at / L, i = at % L;
+    bf16_t* dst = is_k ? a.k : a.v;
+    if (!dst) continue;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (row >= 0) {
+      const int64_t r = row + (int64_t)h * a.kv.P;
+      const uint8_t* src = is_k ? a.kv.k : a.kv.v;
+      o = a.kv.bits == 16 ? __ldg(reinterpret_cast<const uint4*>(src + (r * D + 8 * i) * 2))
+                          : paged_dequant8(a.kv.bits, src, is_k ? a.kv.ks : a.kv.vs, is_k ? a.kv.kb : a.kv.vb, r, D, i);
+    }
+    *reinterpret_cast<uint4*>(dst + (int64_t)t * n * 8 + 8 * at) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention, few query rows per KV head.
+//
+// The G query heads of a KV head times its sequence's new tokens are rows
+// r = t*G + g, tiled by 16: one m16 MMA row tile, so a tile's rows share one
+// pass over the sequence's rows of that head.  Bound by the cache bytes.
+//
+// Work split: an item is (sequence, head, tile); its key range is cut into
+// blocks of 64 keys, and the blocks of all items, laid end to end, are divided
+// evenly over the CTAs of one wave.  So the split follows the true lengths
+// (read on the device), a batch of one long and many short sequences stays
+// balanced, and a CTA leaves at most two partial results (its first and its
+// last item); paged_combine_kernel joins them in CTA order, so a result
+// depends on the lengths and the device's SM count alone.
+//
+// Within a block each of the four warps takes 16 keys and runs its own
+// online softmax; the warps meet once per item, in shared memory.  K and V
+// go from global memory straight to MMA fragments: the contraction order of
+// q.k is free, so a lane's B fragments are 8 (16 when quantized) consecutive
+// values of a key, Q being laid out the same way; and the output column
+// order is free, so a lane's V fragments are 8 consecutive values of four
+// keys, paired by byte permutes.  The next block's K loads are issued when the
+// scores are done, its V loads when P V is done, so loads stay in flight
+// through the arithmetic without a second set of registers.
+//
+// Precision: scores and sums fp32; p enters P V as two bf16 terms
+// p_hi = bf16(p), p_lo = bf16(p - p_hi) (17 significant bits) because one term
+// would double the output's rounding error and the tensor pipe is idle enough
+// for both.  Quantized caches: codes enter the MMAs exactly and scale / bias are applied
+// outside, per group of 64 head dims,
+//   q.k = sum_g s_g (q_g . c_g) + b_g sum q_g,
+//   sum_j p_j v_j = sum_j (p_j s_j) (c_j - z) + sum_j p_j (b_j + z s_j),
+// z = 8 or 128 being the middle of the code range, so that the first sum
+// does not cancel against the second.
+// ---------------------------------------------------------------------------
+static constexpr int kPagedKeys = 64;  // keys per block
+
+struct PagedAttnArgs {
+  PagedKv kv;
+  PagedBatch b;
+  const bf16_t* q;
+  int64_t ldq;
+  int heads, G;
+  float scale2;  // scale * log2(e): the softmax runs in base 2
+  int window;
+  bf16_t* out;
+  int64_t ldo;
+  float* lse;
+  int64_t* prefix;  // scratch: blocks before each sequence [seqs + 1]
+  float* ml;        // [2 * grid][16][2]
+  float* part;      // [2 * grid][16][D]
+  int nctas;
+  unsigned* err;
+};
+
+struct PagedSpan {  // a sequence's work
+  int first, nnew, len, lo;  // packed token, new tokens, rows, first key (page-slot aligned to 16)
+  int tiles, nblk;
+};
+LMX_DEV PagedSpan paged_span(const PagedAttnArgs& a, int s) {
+  PagedSpan z;
+  const int q0 = min(max(__ldg(a.b.q_start + s), 0), a.b.tokens);
+  const int q1 = min(__ldg(a.b.q_start + s + 1), a.b.tokens);
+  z.first = q0;
+  z.nnew = max(q1 - q0, 0);
+  const int64_t cap = (int64_t)a.b.table_stride << a.kv.logP;
+  z.len = (int)min((int64_t)max(__ldg(a.b.kv_len + s), 0), cap);
+  z.lo = 0;
+  if (a.window > 0) z.lo = max(0, __ldg(a.b.kv_len + s) - z.nnew - a.window + 1) & ~15;
+  z.tiles = (int)(((int64_t)z.nnew * a.G + 15) / 16);
+  z.nblk = max(1, (max(z.len - z.lo, 0) + kPagedKeys - 1) / kPagedKeys);
+  return z;
+}
+LMX_DEV int64_t paged_span_blocks(const PagedAttnArgs& a, const PagedSpan& z) {
+  return (int64_t)z.tiles * z.nblk * a.kv.Hk;
+}
+
+// blocks before each sequence, by the whole CTA (128 threads) into shared memory
+LMX_DEV void paged_prefix(const PagedAttnArgs& a, int64_t* pre, int64_t* wsum) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t carry = 0;
+  if (tid == 0) pre[0] = 0;
+  for (int base = 0; base < a.b.seqs; base += 128) {
+    int64_t v = 0;
+    if (base + tid < a.b.seqs) v = paged_span_blocks(a, paged_span(a, base + tid));
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, v, off);
+      if (lane >= off) v += o;
+    }
+    if (lane == 31) wsum[warp] = v;
+    __syncthreads();
+    int64_t before = carry;
+    for (int w = 0; w < warp; ++w) before += wsum[w];
+    if (base + tid < a.b.seqs) pre[base + tid + 1] = before + v;
+    for (int w = 0; w < 4; ++w) carry += wsum[w];
+    __syncthreads();
+  }
+  __syncthreads();
+}
+
+template <int D, int BITS>
+struct PagedFrag {
+  static constexpr int NG = D / 64;
+  static constexpr int KW = BITS == 16 ? D / 8 : (BITS == 8 ? D / 16 : D / 32);  // words of one key's lane share
+  static constexpr int VW = BITS == 16 ? D / 16 : (BITS == 8 ? D / 32 : D / 64);  // words of one V row's lane share
+  uint32_t k[2][KW];
+  uint32_t v[4][VW];
+  uint32_t ks[2][NG], kb[2][NG], vs[2][NG], vb[2][NG];  // bf16 pairs (quantized)
+};
+
+template <int N>
+LMX_DEV void ld_words(uint32_t* d, const uint8_t* p) {
+  if constexpr (N == 4) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+    d[0] = w.x; d[1] = w.y; d[2] = w.z; d[3] = w.w;
+  } else if constexpr (N == 2) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+    d[0] = w.x; d[1] = w.y;
+  } else {
+    d[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+
+// K fragments (and the quantizer's scales and biases) of the 16 keys whose
+// first row is `row`; keys past `n` are not read (their scores are masked).
+template <int D, int BITS>
+LMX_DEV void paged_load_k(PagedFrag<D, BITS>& f, const PagedKv& kv, int64_t row, int n, int g, int c) {
+  using F = PagedFrag<D, BITS>;
+  constexpr int RB = D * BITS / 8;               // bytes of a row
+  constexpr int CH = BITS == 16 ? 64 : 64 * BITS / 8;  // bytes of one chunk (32 values, or a group of 64)
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    const bool there = row >= 0 && 8 * kt + g < n;
+    const uint8_t* p = kv.k + (row + 8 * kt + g) * RB + c * (CH / 4);
+#pragma unroll
+    for (int w = 0; w < F::KW; ++w) f.k[kt][w] = 0;
+    if (there) {
+#pragma unroll
+      for (int i = 0; i < RB / CH; ++i) ld_words<CH / 16>(f.k[kt] + i * (CH / 16), p + i * CH);
+    }
+    if constexpr (BITS != 16) {
+#pragma unroll
+      for (int w = 0; w < F::NG; ++w) f.ks[kt][w] = f.kb[kt][w] = 0;
+      if (row >= 0) {  // whole pages hold 16 scales: rows past n are within the page
+        const int64_t at = (row + 8 * kt + 2 * c) * F::NG;
+        ld_words<F::NG>(f.ks[kt], reinterpret_cast<const uint8_t*>(kv.ks + at));
+        ld_words<F::NG>(f.kb[kt], reinterpret_cast<const uint8_t*>(kv.kb + at));
+      }
+    }
+  }
+}
+// V fragments: rows 2c, 2c+1, 2c+8, 2c+9; rows past n read as zero, whatever
+// the page holds there.
+template <int D, int BITS>
+LMX_DEV void paged_load_v(PagedFrag<D, BITS>& f, const PagedKv& kv, int64_t row, int n, int g, int c) {
+  using F = PagedFrag<D, BITS>;
+  constexpr int RB = D * BITS / 8, CH = RB / (D / 64);  // bytes of 64 values
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int key = 2 * c + (r & 1) + 8 * (r >> 1);
+    const uint8_t* p = kv.v + (row + key) * RB + g * (CH / 8);
+#pragma unroll
+    for (int w = 0; w < F::VW; ++w) f.v[r][w] = 0;
+    if (row >= 0 && key < n)
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) ld_words<CH / 32>(f.v[r] + i * (CH / 32), p + i * CH);
+  }
+  if constexpr (BITS != 16) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int w = 0; w < F::NG; ++w) f.vs[kt][w] = f.vb[kt][w] = 0;
+      if (row >= 0) {
+        const int64_t at = (row + 8 * kt + 2 * c) * F::NG;
+        ld_words<F::NG>(f.vs[kt], reinterpret_cast<const uint8_t*>(kv.vs + at));
+        ld_words<F::NG>(f.vb[kt], reinterpret_cast<const uint8_t*>(kv.vb + at));
+      }
+    }
+  }
+}
+// scale or bias of key 2c+e, group gr, from the packed pairs of one key tile
+template <int NG>
+LMX_DEV float pair_at(const uint32_t (&w)[NG], int e, int gr) {
+  if constexpr (NG == 2) return gr ? hi_bf(w[e]) : lo_bf(w[e]);
+  else return e ? hi_bf(w[0]) : lo_bf(w[0]);
+}
+// two bytes in the low bytes of the 16-bit halves of t -> exact bf16 pair
+// (code - 128): 0x4300 | low seven bits is 128 + them, and the number to
+// subtract is 128 with bit 7 set, 256 without
+LMX_DEV uint32_t code8_pair(uint32_t t) {
+  const uint32_t x = (t & 0x007F007Fu) | 0x43004300u, z = (t & 0x00800080u) ^ 0x43804380u;
+  return bf2_fma3(z, 0xBF80BF80u, x);
+}
+
+template <int D, int BITS>
+__global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedAttnArgs a) {
+  using F = PagedFrag<D, BITS>;
+  constexpr int NG = D / 64, QW = D / 8;  // Q words per lane and row
+  constexpr int OP = D + 4;               // pitch of the merge buffer
+  extern __shared__ int64_t pre[];
+  __shared__ int64_t wsum[4];
+  __shared__ float sm_m[4][16], sm_l[4][16];
+  __shared__ __align__(16) float sm_o[4][16][OP];
+  grid_wait();
+  grid_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+
+  paged_prefix(a, pre, wsum);
+  const int64_t total = pre[a.b.seqs];
+  if (blockIdx.x == 0) {
+    for (int s = tid; s <= a.b.seqs; s += 128) a.prefix[s] = pre[s];
+    for (int s = tid; s < a.b.seqs; s += 128)
+      if (__ldg(a.b.kv_len + s) > ((int64_t)a.b.table_stride << a.kv.logP) &&
+          __ldg(a.b.q_start + s + 1) > __ldg(a.b.q_start + s))
+        atomicExch(a.err, kPagedErr);
+  }
+  const int64_t n = total < a.nctas ? total : a.nctas;
+  if (blockIdx.x >= n) return;
+  int64_t at = total * blockIdx.x / n;
+  const int64_t end = total * (blockIdx.x + 1) / n;
+  int seq = 0;
+  {
+    int hi = a.b.seqs;  // last sequence whose prefix is <= at
+    while (hi - seq > 1) {
+      const int mid = (seq + hi) / 2;
+      if (pre[mid] <= at) seq = mid;
+      else hi = mid;
+    }
+  }
+  bool first_seg = true;
+  while (at < end) {
+    while (pre[seq + 1] <= at) ++seq;
+    const PagedSpan z = paged_span(a, seq);
+    const int64_t loc = at - pre[seq];
+    const int b0 = (int)(loc % z.nblk), tile = (int)(loc / z.nblk % z.tiles), h = (int)(loc / z.nblk / z.tiles);
+    const int b1 = (int)min((int64_t)z.nblk, b0 + (end - at));
+
+    // rows of this lane: g and g + 8 of the tile
+    const int r0 = tile * 16 + g;
+    int klo[2], khi[2];
+    uint32_t qf[2][QW];
+    float qs[2][NG];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = r0 + 8 * k, t = r / a.G;
+      const bool live = t < z.nnew;
+      const int pos = __ldg(a.b.kv_len + seq) - z.nnew + t;
+      khi[k] = live ? min(pos + 1, z.len) : 0;
+      klo[k] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+#pragma unroll
+      for (int w = 0; w < QW; ++w) qf[k][w] = 0;
+      if (live) {
+        const bf16_t* qp = a.q + (int64_t)(z.first + t) * a.ldq + (int64_t)(h * a.G + r % a.G) * D;
+        if constexpr (BITS == 16) {
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) ld_words<4>(qf[k] + 4 * i, reinterpret_cast<const uint8_t*>(qp + 32 * i + 8 * c));
+        } else {
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            ld_words<4>(qf[k] + 8 * i, reinterpret_cast<const uint8_t*>(qp + 64 * i + 16 * c));
+            ld_words<4>(qf[k] + 8 * i + 4, reinterpret_cast<const uint8_t*>(qp + 64 * i + 16 * c + 8));
+          }
+        }
+      }
+      if constexpr (BITS != 16) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) sum += lo_bf(qf[k][8 * i + w]) + hi_bf(qf[k][8 * i + w]);
+          qs[k][i] = warp_sum_xor(sum, 2, 1);
+        }
+      }
+      if constexpr (BITS == 4) {  // a word's nibbles come out as pairs (0,4) (1,5) (2,6) (3,7)
+#pragma unroll
+        for (int w = 0; w < QW; w += 4) {
+          const uint32_t w0 = qf[k][w], w1 = qf[k][w + 1], w2 = qf[k][w + 2], w3 = qf[k][w + 3];
+          qf[k][w] = __byte_perm(w0, w2, 0x5410);
+          qf[k][w + 1] = __byte_perm(w0, w2, 0x7632);
+          qf[k][w + 2] = __byte_perm(w1, w3, 0x5410);
+          qf[k][w + 3] = __byte_perm(w1, w3, 0x7632);
+        }
+      }
+    }
+    float o[NG][8][4];
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][j][e] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, vbs[2][NG] = {};
+
+    // step b: keys [lo + 64 b + 16 warp, +16); its row of head h, or -1
+    auto row_of = [&](int b, int& cnt) -> int64_t {
+      const int key = z.lo + b * kPagedKeys + warp * 16;
+      cnt = z.len - key;
+      if (b >= b1 || cnt <= 0) return -1;
+      const int64_t r = paged_row(a.kv, a.b, seq, key);
+      if (r < 0 && lane == 0) atomicExch(a.err, kPagedErr);
+      return r < 0 ? -1 : r + (int64_t)h * a.kv.P;
+    };
+    F f;
+    int cnt;
+    int64_t row = row_of(b0, cnt);
+    paged_load_k<D, BITS>(f, a.kv, row, cnt, g, c);
+    paged_load_v<D, BITS>(f, a.kv, row, cnt, g, c);
+    for (int b = b0; b < b1; ++b) {
+      int ncnt;
+      const int64_t nrow = row_of(b + 1, ncnt);
+      float s[2][4];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        if constexpr (BITS == 16) {
+          s[kt][0] = s[kt][1] = s[kt][2] = s[kt][3] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < QW; w += 2)
+            mma_bf16(s[kt], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], f.k[kt][w], f.k[kt][w + 1]);
+        } else {
+          float sg[NG][4] = {};
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // k16 steps of the group
+              uint32_t k0, k1;
+              if constexpr (BITS == 8) {
+                const uint32_t w = f.k[kt][4 * i + j];
+                k0 = code8_pair(__byte_perm(w, 0, 0x4140));
+                k1 = code8_pair(__byte_perm(w, 0, 0x4342));
+              } else {  // exact 128 + code
+                const uint32_t w = f.k[kt][2 * i + (j >> 1)] >> (8 * (j & 1));
+                k0 = (w & 0x000F000Fu) | 0x43004300u;
+                k1 = ((w >> 4) & 0x000F000Fu) | 0x43004300u;
+              }
+              const int w = 8 * i + 2 * j;
+              mma_bf16(sg[i], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], k0, k1);
+            }
+          }
+          constexpr float Z = BITS == 8 ? 128.0f : -128.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[kt][e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+              const float sc = pair_at<NG>(f.ks[kt], e & 1, i), bi = __fmaf_rn(Z, sc, pair_at<NG>(f.kb[kt], e & 1, i));
+              s[kt][e] = __fmaf_rn(sc, sg[i][e], __fmaf_rn(bi, qs[e >> 1][i], s[kt][e]));
+            }
+          }
+        }
+      }
+      paged_load_k<D, BITS>(f, a.kv, nrow, ncnt, g, c);
+
+      // scores in base 2; keys a row does not see at -infinity
+      const int key = z.lo + b * kPagedKeys + warp * 16 + 2 * c;
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = key + 8 * kt + (e & 1), k = e >> 1;
+          s[kt][e] = j < khi[k] && j >= klo[k] ? __fmul_rn(s[kt][e], a.scale2) : -INFINITY;
+          mx[k] = fmaxf(mx[k], s[kt][e]);
+        }
+      float msafe[2];
+      bool grow = false;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
+        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
+        mx[k] = fmaxf(mx[k], m[k]);
+        grow = grow || mx[k] != m[k];
+        msafe[k] = mx[k] == -INFINITY ? 0.0f : mx[k];
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float al = ex2f(m[k] - msafe[k]);
+          m[k] = mx[k];
+          l[k] *= al;
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            vbs[k][i] *= al;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              o[i][j][2 * k] *= al;
+              o[i][j][2 * k + 1] *= al;
+            }
+          }
+        }
+      }
+      float p[2][4];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[kt][e] = ex2f(s[kt][e] - msafe[e >> 1]);
+          l[e >> 1] += p[kt][e];
+        }
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        // A fragments: a0 (row g, keys 0..7) a1 (row g+8) a2 (row g, keys 8..15) a3
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float x0 = p[kt][2 * k], x1 = p[kt][2 * k + 1];
+            if constexpr (BITS != 16) {
+              constexpr float Z = BITS == 8 ? 128.0f : 8.0f;
+              const float s0 = pair_at<NG>(f.vs[kt], 0, i), s1 = pair_at<NG>(f.vs[kt], 1, i);
+              // a key that the row does not see has p = 0 and may hold any scale
+              if (x0 != 0.0f) {
+                vbs[k][i] = __fmaf_rn(x0, __fmaf_rn(Z, s0, pair_at<NG>(f.vb[kt], 0, i)), vbs[k][i]);
+                x0 *= s0;
+              }
+              if (x1 != 0.0f) {
+                vbs[k][i] = __fmaf_rn(x1, __fmaf_rn(Z, s1, pair_at<NG>(f.vb[kt], 1, i)), vbs[k][i]);
+                x1 *= s1;
+              }
+            }
+            const uint32_t hi = pk_bf2(x0, x1);
+            ph[2 * kt + k] = hi;
+            pl[2 * kt + k] = pk_bf2(x0 - lo_bf(hi), x1 - hi_bf(hi));
+          }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t vv[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if constexpr (BITS == 16) {
+              vv[k] = __byte_perm(f.v[2 * k][4 * i + j / 2], f.v[2 * k + 1][4 * i + j / 2], (j & 1) ? 0x7632 : 0x5410);
+            } else if constexpr (BITS == 8) {
+              vv[k] = code8_pair(__byte_perm(f.v[2 * k][2 * i + j / 4], f.v[2 * k + 1][2 * i + j / 4],
+                                             (j & 3) | ((4 + (j & 3)) << 8)));
+            } else {  // code - 8
+              const uint32_t t = __byte_perm(f.v[2 * k][i], f.v[2 * k + 1][i], j < 4 ? 0x5410 : 0x7632) >> (4 * (j & 3));
+              vv[k] = bf2_fma3((t & 0x000F000Fu) | 0x43004300u, 0x3F803F80u, 0xC308C308u);
+            }
+          }
+          mma_bf16(o[i][j], ph[0], ph[1], ph[2], ph[3], vv[0], vv[1]);
+          mma_bf16(o[i][j], pl[0], pl[1], pl[2], pl[3], vv[0], vv[1]);
+        }
+      }
+      paged_load_v<D, BITS>(f, a.kv, nrow, ncnt, g, c);
+      row = nrow;
+      cnt = ncnt;
+    }
+
+    // the four warps' results meet: sums over the lanes of a row, then
+    // exp-weighted sums over the warps
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      l[k] = warp_sum_xor(l[k], 2, 1);
+      if constexpr (BITS != 16) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) vbs[k][i] = warp_sum_xor(vbs[k][i], 2, 1);
+      }
+      if (c == 0) {
+        sm_m[warp][g + 8 * k] = m[k];
+        sm_l[warp][g + 8 * k] = l[k];
+      }
+      // lane (g, c) holds columns 64 i + 16 c .. + 15 of its rows
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int j = 0; j < 8; j += 4)
+            *reinterpret_cast<float4*>(&sm_o[warp][g + 8 * k][64 * i + 16 * c + 8 * half + j]) =
+                make_float4(o[i][j][2 * k + half] + vbs[k][i], o[i][j + 1][2 * k + half] + vbs[k][i],
+                            o[i][j + 2][2 * k + half] + vbs[k][i], o[i][j + 3][2 * k + half] + vbs[k][i]);
+    }
+    __syncthreads();
+    {
+      const int row16 = tid >> 3, col = (tid & 7) * (D / 8);
+      float M = -INFINITY, L = 0.0f, w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) M = fmaxf(M, sm_m[k][row16]);
+      const float ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[k] = ex2f(sm_m[k][row16] - ms);
+        L = __fmaf_rn(w[k], sm_l[k][row16], L);
+      }
+      float acc[D / 8];
+#pragma unroll
+      for (int d = 0; d < D / 8; d += 4) {
+        float4 s4 = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(&sm_o[k][row16][col + d]);
+          s4.x = __fmaf_rn(w[k], x.x, s4.x);
+          s4.y = __fmaf_rn(w[k], x.y, s4.y);
+          s4.z = __fmaf_rn(w[k], x.z, s4.z);
+          s4.w = __fmaf_rn(w[k], x.w, s4.w);
+        }
+        acc[d] = s4.x; acc[d + 1] = s4.y; acc[d + 2] = s4.z; acc[d + 3] = s4.w;
+      }
+      const int r = tile * 16 + row16, t = r / a.G;
+      if (t < z.nnew) {
+        if (b0 == 0 && b1 == z.nblk) {
+          const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+          const int head = h * a.G + r % a.G;
+          bf16_t* op = a.out + (int64_t)(z.first + t) * a.ldo + (int64_t)head * D + col;
+#pragma unroll
+          for (int d = 0; d < D / 8; d += 8) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = acc[d + e] * inv;
+            *reinterpret_cast<uint4*>(op + d) = bf8_pack(y);
+          }
+          if (a.lse && (tid & 7) == 0)
+            a.lse[(int64_t)(z.first + t) * a.heads + head] =
+                L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+        } else {
+          const int64_t slot = 2 * (int64_t)blockIdx.x + (first_seg ? 0 : 1);
+          float* pp = a.part + (slot * 16 + row16) * D + col;
+#pragma unroll
+          for (int d = 0; d < D / 8; d += 4) *reinterpret_cast<float4*>(pp + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+          if ((tid & 7) == 0) *reinterpret_cast<float2*>(a.ml + (slot * 16 + row16) * 2) = make_float2(M, L);
+        }
+      }
+    }
+    __syncthreads();
+    first_seg = false;
+    at += b1 - b0;
+  }
+}
+
+// Join of the items that several CTAs share: a warp per (token, head).  The
+// contributors of blocks [i0, i1) are CTAs c0 .. c1; only c0 can have begun
+// in an earlier item (its slot 1), the others begin inside this one.
+template <int D>
+__global__ void __launch_bounds__(128) paged_combine_kernel(PagedAttnArgs a) {
+  grid_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (w >= (int64_t)a.b.tokens * a.heads) return;
+  const int t = (int)(w / a.heads), head = (int)(w % a.heads);
+  const int seq = paged_seq(a.b, t, lane);
+  if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;
+  const PagedSpan z = paged_span(a, seq);
+  const int h = head / a.G, r = (t - z.first) * a.G + head % a.G;
+  const int64_t total = a.prefix[a.b.seqs], n = total < a.nctas ? total : a.nctas;
+  const int64_t i0 = a.prefix[seq] + ((int64_t)h * z.tiles + r / 16) * z.nblk, i1 = i0 + z.nblk;
+  // CTA c owns blocks [total*c/n, total*(c+1)/n)
+  const int64_t c0 = ((i0 + 1) * n - 1) / total, c1 = (i1 * n - 1) / total;
+  if (c0 == c1) return;  // written by its CTA
+  auto slot_of = [&](int64_t cta) { return 2 * cta + (cta == c0 && total * cta / n < i0 ? 1 : 0); };
+  float M = -INFINITY;
+  for (int64_t k = c0 + lane; k <= c1; k += 32) M = fmaxf(M, a.ml[(slot_of(k) * 16 + r % 16) * 2]);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  const float ms = M == -INFINITY ? 0.0f : M;
+  constexpr int V = D / 32;
+  float L = 0.0f, acc[V] = {};
+#pragma unroll 4
+  for (int64_t k = c0; k <= c1; ++k) {
+    const int64_t s = slot_of(k) * 16 + r % 16;
+    const float2 ml = *reinterpret_cast<const float2*>(a.ml + s * 2);
+    const float wt = ex2f(ml.x - ms);
+    L = __fmaf_rn(wt, ml.y, L);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(a.part + s * D + lane * V + e);
+      acc[e] = __fmaf_rn(wt, x.x, acc[e]);
+      acc[e + 1] = __fmaf_rn(wt, x.y, acc[e + 1]);
+    }
+  }
+  const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+  bf16_t* op = a.out + (int64_t)t * a.ldo + (int64_t)head * D + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(op + e) = pk_bf2(acc[e] * inv, acc[e + 1] * inv);
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)t * a.heads + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+}
+
+}  // namespace lmx

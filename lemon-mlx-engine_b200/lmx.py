@@ -23,6 +23,33 @@ class LmxError(RuntimeError):
     pass
 
 
+class PagedKvDesc(C.Structure):
+    """lmx_paged_kv"""
+    _fields_ = [("pages", I), ("page_size", I), ("kv_heads", I), ("head_dim", I), ("bits", I),
+                ("page_stride", I64), ("k", P), ("v", P), ("k_packed", P), ("v_packed", P), ("k_scales", P),
+                ("k_biases", P), ("v_scales", P), ("v_biases", P)]
+
+
+class PagedBatch(C.Structure):
+    """lmx_paged_batch"""
+    _fields_ = [("seqs", I), ("tokens", I), ("max_new", I), ("q_start", P), ("kv_len", P),
+                ("block_table", P), ("table_stride", I)]
+
+
+class RopeDesc(C.Structure):
+    """lmx_rope"""
+    _fields_ = [("cos", P), ("sin", P), ("positions", I), ("rot_dim", I), ("interleaved", I)]
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
+
+
+class RopeScaling(C.Structure):
+    """lmx_rope_scaling"""
+    _fields_ = [("kind", I), ("theta", C.c_double), ("factor", C.c_double), ("low", C.c_double),
+                ("high", C.c_double), ("orig_positions", C.c_double), ("attn_factor", C.c_double)]
+
+
 # Every exported symbol of include/lmx.h with (restype, argtypes).
 SIGNATURES = {
     "lmx_last_error": (C.c_char_p, []),
@@ -53,6 +80,14 @@ SIGNATURES = {
     "lmx_kv_append": (I, [P, P, P, I, P]),
     "lmx_kv_set_position": (I, [P, I, I, P]),
     "lmx_cache_kv": (I, [P, I, P]),
+    "lmx_rope_table": (I, [C.POINTER(RopeScaling), I, I, P, P, P]),
+    "lmx_rope_apply": (I, [C.POINTER(RopeDesc), P, I64, P, I, I, I, I, P, I64, P]),
+    "lmx_paged_append": (I, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatch), C.POINTER(RopeDesc), P, P, P, I64, I,
+                             P, P, F, P, I64, P]),
+    "lmx_paged_gather": (I, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatch), P, P, P]),
+    "lmx_paged_attention_scratch_bytes": (C.c_size_t, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatch), I]),
+    "lmx_paged_attention": (I, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatch), P, I64, I, F, I, P, C.c_size_t, P,
+                                I64, P, P]),
     "lmx_model_create": (I, [P, U64, P]),
     "lmx_model_create_tp": (I, [P, U64, P, P]),
     "lmx_model_config_load": (I, [C.c_char_p, P, P, I, P]),

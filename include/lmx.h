@@ -329,7 +329,7 @@ int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* batch, void*
 /* Attention of the new tokens over the cache (their own rows already
  * appended): the token at position p of its sequence sees the cached rows
  * max(0, p - window + 1) .. p (window 0: all up to p);
- *   out = softmax(scale * q.k) v,   lse = ln sum exp(scale * q.k).
+ *   out = softmax(scale * q.k) v,   lse = ln sum exp(scale * q.k),   scale > 0.
  * q, out [tokens][heads][head_dim] bf16, token rows ldq / ldo values apart
  * (out must not overlap q); lse fp32 [tokens][heads] or NULL.  heads is a
  * multiple of kv_heads, at most 64 times it.  A row that sees nothing gives
@@ -343,6 +343,12 @@ size_t lmx_paged_attention_scratch_bytes(const lmx_paged_kv* kv, const lmx_paged
 int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch* batch, const void* q, int64_t ldq, int heads,
                         float scale, int window, void* scratch, size_t scratch_bytes, void* out, int64_t ldo,
                         float* lse, void* stream);
+/* Query rows per KV head (max_new * heads / kv_heads) from which
+ * lmx_paged_attention takes the tcgen05 prompt kernel; below it, and with 0
+ * always, the few-row kernel.  Scratch sizes follow it.  Process-wide; no
+ * reference counterpart. */
+int lmx_set_paged_prompt_min_rows(int rows);
+int lmx_paged_prompt_min_rows(void);
 
 /* ---------------------------------------------------------------------------
  * Hybrid-model ops (configuration 4, Qwen3-Next-style decoder).

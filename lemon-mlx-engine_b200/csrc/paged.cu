@@ -4,7 +4,10 @@
 #include <cstring>
 
 #include "lmx_internal.h"
+#include <cudaTypedefs.h>
+
 #include "paged.cuh"
+#include "paged_prompt.cuh"
 
 using namespace lmx;
 
@@ -235,9 +238,14 @@ extern "C" int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* b
 // ---------------------------------------------------------------------------
 namespace {
 
+// Query rows per KV head (max_new * heads / kv_heads) from which the prompt
+// kernel runs; 0: never.
+int g_prompt_min_rows = 33;
+
 struct AttnPlan {
+  bool prompt = false;
   int nctas = 0;
-  size_t prefix = 0, ml = 0, part = 0, bytes = 0;  // offsets into the scratch
+  size_t start = 0, ml = 0, part = 0, bytes = 0;  // offsets into the scratch
 };
 
 template <int D, int BITS>
@@ -268,13 +276,87 @@ int check_attn(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads, 
     return set_error(LMX_ERR_UNSUPPORTED, "paged_attention: heads=%d over kv_heads=%d (a multiple, at most 64 times)",
                      heads, kv->kv_heads);
   const int D = kv->head_dim;
-  if (D == 64) rc = kv->bits == 16 ? few_rows_ctas<64, 16>(&p.nctas) : kv->bits == 8 ? few_rows_ctas<64, 8>(&p.nctas) : few_rows_ctas<64, 4>(&p.nctas);
-  else rc = kv->bits == 16 ? few_rows_ctas<128, 16>(&p.nctas) : kv->bits == 8 ? few_rows_ctas<128, 8>(&p.nctas) : few_rows_ctas<128, 4>(&p.nctas);
+  p.prompt = kv->bits == 16 && g_prompt_min_rows > 0 &&
+             (int64_t)batch->max_new * (heads / kv->kv_heads) >= g_prompt_min_rows;
+  int rows = 16;  // of a partial result
+  if (p.prompt) {
+    rows = kPromptRows;
+    p.nctas = device_sms();
+  } else if (D == 64) {
+    rc = kv->bits == 16 ? few_rows_ctas<64, 16>(&p.nctas) : kv->bits == 8 ? few_rows_ctas<64, 8>(&p.nctas) : few_rows_ctas<64, 4>(&p.nctas);
+  } else {
+    rc = kv->bits == 16 ? few_rows_ctas<128, 16>(&p.nctas) : kv->bits == 8 ? few_rows_ctas<128, 8>(&p.nctas) : few_rows_ctas<128, 4>(&p.nctas);
+  }
   if (rc) return rc;
-  p.ml = ((size_t)(batch->seqs + 1) * 8 + 255) / 256 * 256;
-  p.part = p.ml + (size_t)2 * p.nctas * 16 * 2 * 4;
-  p.bytes = p.part + (size_t)2 * p.nctas * 16 * D * 4;
+  auto after = [](size_t at, size_t bytes) { return (at + bytes + 255) / 256 * 256; };
+  p.start = after(0, (size_t)(batch->seqs + 1) * 8);
+  p.ml = after(p.start, p.prompt ? (size_t)p.nctas * sizeof(int4) : 0);
+  p.part = after(p.ml, (size_t)2 * p.nctas * rows * 2 * 4);
+  p.bytes = p.part + (size_t)2 * p.nctas * rows * D * 4;
   return LMX_OK;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
+    return (PFN_cuTensorMapEncodeTiled_v12000)f;
+  }();
+  return fn;
+}
+
+// bf16 map of `rank` dimensions, 128-byte swizzle, boxes of 64 values in the
+// first; strides in values
+int tensor_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides,
+               const cuuint32_t* box) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return set_error(LMX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t st[3];
+  for (int i = 0; i + 1 < rank; ++i) st[i] = (cuuint64_t)strides[i] * 2;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, st, box, one,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(LMX_ERR_INVALID, "paged_attention: tensor map encode failed (%d)", (int)r);
+  return LMX_OK;
+}
+
+template <int D>
+int launch_prompt(const PagedAttnArgs& a, const AttnPlan& pl, cudaStream_t st) {
+  PromptArgs p;
+  p.a = a;
+  p.TT = 128 / a.G;
+  p.start = (int4*)((uint8_t*)a.prefix + pl.start);
+  PromptMaps mp;
+  const cuuint64_t qd[3] = {D, (cuuint64_t)a.heads, (cuuint64_t)a.b.tokens};
+  const int64_t qs[2] = {D, a.ldq};
+  const cuuint32_t qb[3] = {64, (cuuint32_t)a.G, (cuuint32_t)p.TT};
+  int rc = tensor_map(&mp.q, a.q, 3, qd, qs, qb);
+  const cuuint64_t kd[4] = {D, (cuuint64_t)a.kv.P, (cuuint64_t)a.kv.Hk, (cuuint64_t)a.kv.pages};
+  const int64_t ks[3] = {D, (int64_t)a.kv.P * D, a.kv.pstride * D};
+  const cuuint32_t kb[4] = {64, (cuuint32_t)(a.kv.P < 128 ? a.kv.P : 128), 1, 1};
+  if (!rc) rc = tensor_map(&mp.k, a.kv.k, 4, kd, ks, kb);
+  if (!rc) rc = tensor_map(&mp.v, a.kv.v, 4, kd, ks, kb);
+  if (rc) return rc;
+  static bool attr_set[64] = {};
+  int d = 0;
+  cudaGetDevice(&d);
+  constexpr int smem = PromptSmem<D>::BYTES;
+  if (!attr_set[d & 63]) {
+    rc = cuda_check(cudaFuncSetAttribute(paged_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                    "paged_attention: set smem");
+    if (rc) return rc;
+    attr_set[d & 63] = true;
+  }
+  rc = cuda_check(lmx_launch(paged_prompt_plan_kernel, dim3(1), dim3(1024), 0, st, true, p), "paged_attention: plan launch");
+  if (!rc)
+    rc = cuda_check(lmx_launch(paged_prompt_kernel<D>, dim3(a.nctas), dim3(kPromptThreads), smem, st, true, mp, p),
+                    "paged_attention: prompt launch");
+  if (!rc)
+    rc = cuda_check(lmx_launch(paged_prompt_join_kernel<D>, dim3(a.nctas, kPromptRows / 32), dim3(128), 0, st, true, p),
+                    "paged_attention: join launch");
+  return rc;
 }
 
 template <int D, int BITS>
@@ -289,6 +371,13 @@ int launch_few(const PagedAttnArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+extern "C" int lmx_set_paged_prompt_min_rows(int rows) {
+  if (rows < 0) return set_error(LMX_ERR_INVALID, "paged_prompt_min_rows %d", rows);
+  g_prompt_min_rows = rows;
+  return LMX_OK;
+}
+extern "C" int lmx_paged_prompt_min_rows(void) { return g_prompt_min_rows; }
 
 extern "C" size_t lmx_paged_attention_scratch_bytes(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads) {
   AttnPlan p;
@@ -307,7 +396,8 @@ extern "C" int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch
     return set_error(LMX_ERR_INVALID,
                      "paged_attention: q and out must be 16-byte aligned, rows a multiple of 8 values and at least "
                      "heads * head_dim apart");
-  if (window < 0) return set_error(LMX_ERR_INVALID, "paged_attention: window=%d", window);
+  if (window < 0 || !(scale > 0) || std::isinf(scale))
+    return set_error(LMX_ERR_INVALID, "paged_attention: window=%d scale=%g (a positive number)", window, scale);
   if (!scratch || !aligned16(scratch) || scratch_bytes < p.bytes)
     return set_error(LMX_ERR_INVALID, "paged_attention: needs %zu bytes of 16-byte aligned scratch (%zu given)", p.bytes,
                      scratch_bytes);
@@ -329,6 +419,7 @@ extern "C" int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch
   a.nctas = p.nctas;
   a.err = device_error_word();
   cudaStream_t st = (cudaStream_t)stream;
+  if (p.prompt) return D == 64 ? launch_prompt<64>(a, p, st) : launch_prompt<128>(a, p, st);
   if (D == 64)
     return kv->bits == 16 ? launch_few<64, 16>(a, st) : kv->bits == 8 ? launch_few<64, 8>(a, st) : launch_few<64, 4>(a, st);
   return kv->bits == 16 ? launch_few<128, 16>(a, st) : kv->bits == 8 ? launch_few<128, 8>(a, st) : launch_few<128, 4>(a, st);

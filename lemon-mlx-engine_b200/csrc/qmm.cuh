@@ -33,6 +33,7 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include "lmx_common.cuh"
+#include "sm100.cuh"
 #include "norm_argmax.cuh"
 namespace cg = cooperative_groups;
 
@@ -75,70 +76,6 @@ struct QmmMaps {
 static constexpr int kQmmThreads = 256;
 static constexpr int kQmmMaxNormRows = 64;
 
-LMX_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-LMX_DEV void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-LMX_DEV void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-               "r"(bytes)
-               : "memory");
-}
-LMX_DEV void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
-LMX_DEV bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-#ifdef LMX_MBAR_POLL
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-#else
-  // suspend-time hint 1 ms: the thread sleeps in hardware until the phase
-  // completes (or the hint expires) instead of spinning on issue slots
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
-      : "memory");
-#endif
-  return ok != 0;
-}
-LMX_DEV uint64_t global_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-// Bounded wait: gives up after 4 s of wall time or 2^26 polls, whichever
-// comes first, and flags the error word.  The polling loop is out of line so
-// that the common case (phase already complete) stays a few instructions,
-// and it backs off with nanosleep (32 ns doubling to 256 ns): warps that run
-// ahead of a pipeline would otherwise spin and take issue slots from the
-// warps whose work they are waiting for.
-__device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
-  const uint64_t t0 = global_ns();
-  uint32_t ns = 32;
-  for (uint32_t i = 1; i < (1u << 26); ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    __nanosleep(ns);
-    if (ns < 256) ns <<= 1;
-    if (global_ns() - t0 > 4000000000ull) break;
-  }
-  if (err) atomicExch(err, code);
-  return false;
-}
-LMX_DEV bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait_slow(bar, parity, err, code);
-}
-
 // Item -> (matrix, row).  PLAIN/RESID: items are the concatenated rows of
 // mat[0..nmat).  SWIGLU: a batch of RB items holds RB/2 gate rows followed by
 // the same RB/2 up rows, so both runs are contiguous in memory and in smem.
@@ -161,13 +98,6 @@ LMX_DEV bool qmm_item_row(const QmmArgs& a, int item, int& mi, int& row) {
   return false;
 }
 
-LMX_DEV void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
 
 LMX_DEV const QmmMat& qmm_mat(const QmmArgs& a, int mi) {
   return mi == 0 ? a.mat[0] : (mi == 1 ? a.mat[1] : a.mat[2]);

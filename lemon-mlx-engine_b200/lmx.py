@@ -88,6 +88,8 @@ SIGNATURES = {
     "lmx_paged_attention_scratch_bytes": (C.c_size_t, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatch), I]),
     "lmx_paged_attention": (I, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatch), P, I64, I, F, I, P, C.c_size_t, P,
                                 I64, P, P]),
+    "lmx_set_paged_prompt_min_rows": (I, [I]),
+    "lmx_paged_prompt_min_rows": (I, []),
     "lmx_model_create": (I, [P, U64, P]),
     "lmx_model_create_tp": (I, [P, U64, P, P]),
     "lmx_model_config_load": (I, [C.c_char_p, P, P, I, P]),

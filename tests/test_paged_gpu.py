@@ -332,6 +332,48 @@ def test_attention_few_rows(lmx, cuda, bits, lens, hk, g, d, page, window):
     check(cache, q, got, lse, d ** -0.5, window)
 
 
+@pytest.fixture
+def prompt_rows(lmx):
+    """Set the row count from which the prompt kernel runs; restores the default."""
+    before = lmx.lib().lmx_paged_prompt_min_rows()
+    yield lambda n: lmx.call("lmx_set_paged_prompt_min_rows", n)
+    lmx.call("lmx_set_paged_prompt_min_rows", before)
+
+
+PROMPT = {"one": [(1, 1)], "prompt": [(200, 200)], "tile edges": [(128, 128), (129, 129), (127, 256), (64, 64), (32, 383)],
+          "ragged": [(150, 300), (0, 40), (1, 131), (2, 2), (0, 0), (77, 640), (1, 1), (300, 301)],
+          "empty rows": [(40, 20), (30, 0), (2, 66), (1, 0), (200, 10)], "long": [(40, 3000)],
+          "mixed": [(1, 700), (90, 1200), (1, 17), (1, 128), (5, 129)]}
+
+
+# rows at the 128-key tile's and the page's ends, every grouping (rows of a
+# tile that 128 / G does not fill), windows that end inside a tile and a page
+@pytest.mark.parametrize("bits", [16])
+@pytest.mark.parametrize("lens,hk,g,d,page,window", [
+    ("one", 1, 1, 128, 16, 0), ("prompt", 2, 1, 64, 32, 0), ("prompt", 1, 4, 128, 128, 0), ("tile edges", 2, 4, 128, 16, 0),
+    ("tile edges", 1, 3, 64, 64, 50), ("tile edges", 1, 1, 128, 256, 128), ("ragged", 2, 4, 128, 32, 0),
+    ("ragged", 1, 7, 64, 128, 33), ("ragged", 3, 2, 128, 256, 1), ("ragged", 2, 5, 128, 64, 200),
+    ("empty rows", 2, 2, 128, 32, 0), ("empty rows", 1, 4, 64, 16, 5), ("long", 1, 8, 128, 16, 0),
+    ("long", 2, 16, 64, 128, 700), ("mixed", 2, 8, 128, 16, 0), ("mixed", 1, 64, 64, 64, 129), ("mixed", 4, 1, 64, 16, 0)])
+def test_attention_prompt_kernel(lmx, cuda, prompt_rows, bits, lens, hk, g, d, page, window):
+    prompt_rows(1)
+    cache = P.Cache(21, PROMPT[lens], hk, d, bits, page, gap=16 if g == 3 else 0, pad=2 if g == 7 else 0)
+    q = (torch.randn((cache.tokens, hk * g, d), generator=cache.gen) * 1.5).to(BF16)
+    P.device_error(lmx)
+    got, lse = attend(lmx, cache, q, hk * g, d ** -0.5, window, extra=8 if g == 2 else 0)
+    assert P.device_error(lmx) == 0
+    # p enters P V as bf16: 2^-8
+    check(cache, q, got, lse, d ** -0.5, window, p_err=2.0 ** -8)
+
+
+def test_attention_prompt_kernel_large_scores(lmx, cuda, prompt_rows):
+    prompt_rows(1)
+    cache = P.Cache(22, [(130, 333), (2, 64)], 2, 128, 16, 32, k_std=8.0)
+    q = (torch.randn((132, 8, 128), generator=cache.gen) * 8).to(BF16)
+    got, lse = attend(lmx, cache, q, 8, 0.25, 0)
+    check(cache, q, got, lse, 0.25, 0, p_err=2.0 ** -8)
+
+
 def test_attention_peaked_and_large_scores(lmx, cuda):
     # one key takes all the weight, and scores far apart (hundreds in the exponent)
     cache = P.Cache(12, [(1, 333), (2, 64)], 2, 128, 16, 32, k_std=8.0)
@@ -395,3 +437,6 @@ def test_attention_rows_past_the_table(lmx, cuda):
     assert lmx.lib().lmx_paged_attention(*args) == 1
     args[6], args[3] = 0, 120
     assert lmx.lib().lmx_paged_attention(*args) == 1
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        args[3], args[5] = 128, scale
+        assert lmx.lib().lmx_paged_attention(*args) == 1

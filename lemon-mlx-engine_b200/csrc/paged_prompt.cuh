@@ -12,10 +12,10 @@
 // tiles of a pair take turns, one in the tensor pipe while the other is in
 // its softmax, so both units stay busy.
 //
-// Warps: 0-3 and 4-7 softmax and epilogue of the pair's first and second tile
-// (a thread owns a row); 8 issues the MMAs; 9 loads (TMA: one box per page and
-// 64 head dims, so the tile in shared memory is the same whatever the page
-// size); 10 follows the loads and clears the V rows of a tile that lie past the
+// Warps: 0-7 and 8-15 softmax and epilogue of the pair's first and second tile
+// (two threads per row, one for each half of the keys and of the head dims);
+// 16 issues the MMAs; 17 loads (TMA: one box per page and 64 head dims, so the
+// tile in shared memory is the same whatever the page size); 18 follows the loads and clears the V rows of a tile that lie past the
 // sequence's end (p = 0 there, but 0 * NaN is not 0).
 // Tensor memory: S of the two tiles [0, 256), O at 256; P (16-bit) overlays
 // the first half of its S, which the softmax has then read.  MMAs issued by
@@ -36,7 +36,8 @@
 
 namespace lmx {
 
-static constexpr int kPromptThreads = 384;
+static constexpr int kPromptSoftmaxWarps = 16;  // per row tile: two halves of four
+static constexpr int kPromptThreads = 32 * kPromptSoftmaxWarps + 128;
 static constexpr int kPromptRows = 256;  // rows of a pair
 
 struct PromptArgs {
@@ -225,12 +226,31 @@ LMX_DEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z,
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
+// One lane of a converged warp.  The MMA warp runs its loop with all lanes, so
+// that descriptors and counters stay in uniform registers (an MMA is then two
+// uniform adds away from the next), and lets one lane issue.
+LMX_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// Descriptors as low words over a constant high word (8-row groups 1024 bytes
+// apart, version 1, 128-byte swizzle): (address >> 4) | leading offset << 16.
+static constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
 // D[tmem] (+)= A[smem] * B[smem]^T
-LMX_DEV void umma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+LMX_DEV void umma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+LMX_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi)
       : "memory");
 }
 LMX_DEV void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -258,35 +278,129 @@ LMX_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: 
 LMX_DEV void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 LMX_DEV void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// V is the B operand with its N index (head dims) contiguous: 64-value blocks
-// of 128 bytes (leading byte offset: from one block of 64 head dims to the
-// next, 128 keys * 128 bytes), 8-key groups 1024 bytes apart.
-LMX_DEV uint64_t umma_desc_v(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// The eight softmax warps of a row tile meet.
+LMX_DEV void prompt_meet(int tile) { asm volatile("bar.sync %0, 256;" ::"r"(1 + tile) : "memory"); }
+
+// ---- the softmax's pieces, on a thread's row of scores ----
+LMX_DEV uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
+LMX_DEV void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+LMX_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+LMX_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+LMX_DEV void prompt_mask(uint32_t* s, int key, int klo, int khi) {
+#pragma unroll
+  for (int i = 0; i < 64; ++i)
+    if (key + i >= khi || key + i < klo) s[i] = 0xff800000u;
+}
+LMX_DEV float prompt_max(const uint32_t* s) {  // of 64, in eight chains
+  float m[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m[k] = __uint_as_float(s[k]);
+#pragma unroll
+  for (int i = 8; i < 56; i += 16)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = fmaxf(fmaxf(m[k], __uint_as_float(s[i + k])), __uint_as_float(s[i + 8 + k]));
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m[k] = fmaxf(m[k], __uint_as_float(s[56 + k]));
+  return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+}
+// 2^x of a pair, x <= 2^8, on the FMA pipe: x = n + f, n the nearest integer
+// (the low bits of x + 1.5 * 2^23), 2^f by a degree-4 polynomial (least
+// maximal relative error over [-1/2, 1/2], 2.6e-6), n added to the exponent.
+// Below 2^-126 it stays there: only rows that see the whole tile come here, so
+// their sum is at least 2^-8.
+LMX_DEV void ex2_pair(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  f2_unpack(x, x0, x1);
+  x = f2_pack(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+  const uint64_t t = f2_add(x, f2_pack(12582912.0f, 12582912.0f));
+  const uint64_t n = f2_add(t, f2_pack(-12582912.0f, -12582912.0f));
+  const uint64_t f = f2_fma(n, f2_pack(-1.0f, -1.0f), x);
+  uint64_t q = f2_pack(0x1.3997d6p-7f, 0x1.3997d6p-7f);
+  q = f2_fma(q, f, f2_pack(0x1.ca1442p-5f, 0x1.ca1442p-5f));
+  q = f2_fma(q, f, f2_pack(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  q = f2_fma(q, f, f2_pack(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  q = f2_fma(q, f, f2_pack(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  float q0, q1, t0, t1;
+  f2_unpack(q, q0, q1);
+  f2_unpack(t, t0, t1);
+  p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
+  p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
+}
+#ifndef EMU
+#define EMU 0
+#endif
+// p = 2^(s * scale2 + ms) of 64 scores, stored as bf16 pairs; returns their sum.
+LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP) {
+  const uint64_t sc = f2_pack(scale2, scale2), mm = f2_pack(ms, ms);
+  uint64_t sum[4] = {};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[32 * h + 2 * i]), __uint_as_float(s[32 * h + 2 * i + 1])), sc, mm);
+      float p0, p1;
+      if (i % 8 >= 8 - EMU) {
+        ex2_pair(x, p0, p1);
+      } else {
+        f2_unpack(x, p0, p1);
+        p0 = ex2f(p0);
+        p1 = ex2f(p1);
+      }
+      sum[i & 3] = f2_add(sum[i & 3], f2_pack(p0, p1));
+      pk[i] = pk_bf2(p0, p1);
+    }
+    tmem_st16(tP + 16 * h, pk);
+  }
+  float a, b;
+  f2_unpack(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])), a, b);
+  return a + b;
+}
+
+// Q and K are K-major (the leading offset is not used within a 128-byte
+// swizzle atom).  V is the B operand with its N index (head dims) contiguous:
+// the leading offset goes from one 64-value block to the next, 128 keys * 128 B.
+static constexpr uint32_t kDescQK = 1u << 16, kDescV = (16384u >> 4) << 16;
 
 template <int D>
 struct PromptSmem {
   static constexpr int TILE = 128 * D * 2;            // one tile of Q, K or V
   static constexpr int NS = D == 128 ? 5 : 8;         // K / V stages
-  static constexpr int BYTES = 2 * TILE + NS * TILE + 1024 + 256;
+  static constexpr int BYTES = 2 * TILE + NS * TILE + 256 + 2048;  // tiles, barriers, exchange
 };
 
 template <int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     paged_prompt_kernel(const __grid_constant__ PromptMaps mp, const __grid_constant__ PromptArgs p) {
   using SM = PromptSmem<D>;
-  constexpr int TILE = SM::TILE, NS = SM::NS, NH = D / 64;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int TILE = SM::TILE, NS = SM::NS, NH = D / 64, kMma = kPromptSoftmaxWarps;
+  // the tiles' swizzle wants 1024-byte alignment: the kernel has no static
+  // shared memory, so the dynamic part begins at a multiple of 1024 (checked)
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) atomicExch(p.a.err, 0x51u);
+    return;
+  }
   uint8_t* Qs = smem;
   uint8_t* KV = smem + 2 * TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(KV + NS * TILE);
   uint64_t *q_full = bars, *q_free = bars + 1, *vfix = bars + 2, *s_full = bars + 3, *p_ready = bars + 5,
            *o_full = bars + 7, *o_free = bars + 9, *drain = bars + 11, *kv_full = bars + 12, *kv_free = kv_full + NS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_free + NS);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* xch = reinterpret_cast<float*>(KV + NS * TILE + 256);  // [tile][half][128]
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -295,17 +409,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     mbar_init(drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_ready + i, 4);
+      mbar_init(p_ready + i, 8);
       mbar_init(o_full + i, 1);
-      mbar_init(o_free + i, 4);
+      mbar_init(o_free + i, 8);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(kv_full + i, 1);
-      mbar_init(kv_free + i, 2);  // the MMAs' commit and warp 10
+      mbar_init(kv_free + i, 2);  // the MMAs' commit and the warp that clears V
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -319,18 +433,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   unsigned* err = p.a.err;
   PromptWalk w;
 
-  if (warp < 8) {
+  if (warp < kPromptSoftmaxWarps) {
     // ------------------------- softmax and epilogue -------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int tile = warp >> 2;  // of the pair
-    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
-    const uint32_t tS = tmem + lanes + tile * 128, tO = tmem + lanes + 256 + tile * D;
-    const int r = (warp & 3) * 32 + lane;               // row of the tile
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int tile = warp >> 3, half = (warp >> 2) & 1;  // of the pair; of the tile's columns
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's 32 TMEM lanes
+    const uint32_t tS = tmem + lanes + tile * 128, tO = tmem + lanes + 256 + tile * D + half * (D / 2);
+    const int r = (warp & 3) * 32 + lane;                // row of the tile
+    float* mine = xch + (tile * 2 + half) * 128 + r;
+    const float* other = xch + (tile * 2 + (half ^ 1)) * 128 + r;
     const int G = p.a.G;
     const float scale2 = p.a.scale2;
     uint32_t ps = 0, po = 0;  // parities of s_full, o_full
     bool ok = true;
-    for (w.begin(p); ok && w.live(); w.next(p)) {
+    // A wait that gives up is the last one; the rest then runs through on
+    // whatever is there, because the halves' barriers need all warps.
+    for (w.begin(p); w.live(); w.next(p)) {
       if (tile == 1 && !w.second(p)) continue;
       const int t = r / G, tok = w.z.t0 + tile * p.TT + t;  // token of the sequence
       const bool row = t < p.TT && tok < w.z.nnew;
@@ -339,33 +457,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       // they do not send their warp through the masks
       const int khi = row ? min(pos + 1, w.z.len) : 1 << 30;
       const int klo = row && p.a.window > 0 ? max(0, pos - p.a.window + 1) : 0;
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f;  // l: this half's
       for (int b = w.b0; b < w.b1; ++b) {
-        ok = prompt_warp_wait(s_full + tile, ps, err, 0x45u);
-        if (!ok) break;
+        ok = ok && prompt_warp_wait(s_full + tile, ps, err, 0x45u);
         ps ^= 1;
         tmem_fence_after();
-        uint32_t s[128];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(tS + 32 * i, s + 32 * i);
+        uint32_t s[64];
+        tmem_ld32(tS + 64 * half, s);
+        tmem_ld32(tS + 64 * half + 32, s + 32);
         tmem_wait_ld();
-        const int key = (w.z.kb + b) << 7;
-        if (!__all_sync(0xffffffffu, key + 128 <= khi && key >= klo)) {
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (key + i >= khi || key + i < klo) s[i] = 0xff800000u;
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) mx = fmaxf(mx, __uint_as_float(s[i]));
-        mx *= scale2;
+        const int key = ((w.z.kb + b) << 7) + 64 * half;
+        if (!__all_sync(0xffffffffu, key + 64 <= khi && key >= klo)) prompt_mask(s, key, klo, khi);
+        const float mh = prompt_max(s);
+        // the two halves of a row agree on its maximum; past this point both
+        // have read their scores, so P may overwrite them
+        // (the other half read the previous one before its P was complete,
+        // and this S came after that P)
+        *mine = mh;
+        tmem_fence_before();
+        prompt_meet(tile);
+        tmem_fence_after();
+        const float mx = fmaxf(mh, *other) * scale2;
         if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
           const float mn = fmaxf(m, mx);
           if (b > w.b0) {
             const float al = mn == -INFINITY ? 1.0f : ex2f(m - mn);
             l *= al;
 #pragma unroll
-            for (int i = 0; i < D; i += 16) {
+            for (int i = 0; i < D / 2; i += 16) {
               float o[16];
               uint32_t u[16];
               tmem_ld16(tO + i, o);
@@ -376,155 +495,148 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
           m = mn;
         }
-        const float ms = m == -INFINITY ? 0.0f : -m;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float p0 = ex2f(__fmaf_rn(__uint_as_float(s[32 * h + 2 * i]), scale2, ms));
-            const float p1 = ex2f(__fmaf_rn(__uint_as_float(s[32 * h + 2 * i + 1]), scale2, ms));
-            sum[i & 1] += p0;
-            sum[2 + (i & 1)] += p1;
-            pk[i] = pk_bf2(p0, p1);
-          }
-          tmem_st16(tS + 16 * h, pk);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += prompt_exp(s, scale2, m == -INFINITY ? 0.0f : -m, tS + 32 * half);
         tmem_wait_st();
         tmem_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready + tile);
       }
-      if (!ok) break;
-      ok = prompt_warp_wait(o_full + tile, po, err, 0x46u);
-      if (!ok) break;
+      ok = ok && prompt_warp_wait(o_full + tile, po, err, 0x46u);
+      // the row's sum from both halves, and once more so that the next item's
+      // maxima do not overtake it
+      *mine = l;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k == 1) l += *other;
+        prompt_meet(tile);
+      }
       po ^= 1;
       tmem_fence_after();
       const int head = w.h * G + r % G;
       if (w.whole()) {
         const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-        bf16_t* op = p.a.out + (int64_t)(w.z.first + tok) * p.a.ldo + (int64_t)head * D;
+        bf16_t* op = p.a.out + (int64_t)(w.z.first + tok) * p.a.ldo + (int64_t)head * D + half * (D / 2);
 #pragma unroll
-        for (int i = 0; i < D; i += 32) {
-          uint32_t o[32];
-          tmem_ld32(tO + i, o);
-          tmem_wait_ld();
+        for (int i = 0; i < D / 2; i += 16) {
+          float o[16];
+          tmem_ld16(tO + i, o);
           if (row)
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
+            for (int k = 0; k < 16; k += 8) {
               float y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[k + e]) * inv;
+              for (int e = 0; e < 8; ++e) y[e] = o[k + e] * inv;
               *reinterpret_cast<uint4*>(op + i + k) = bf8_pack(y);
             }
         }
-        if (row && p.a.lse)
+        if (half == 0 && row && p.a.lse)
           p.a.lse[(int64_t)(w.z.first + tok) * p.a.heads + head] =
               l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
       } else {
         const int64_t slot = 2 * (int64_t)blockIdx.x + (w.first ? 0 : 1);
-        float4* pp = reinterpret_cast<float4*>(p.a.part) + slot * (D / 4) * kPromptRows + tile * 128 + r;
+        float4* pp = reinterpret_cast<float4*>(p.a.part) + (slot * (D / 4) + half * (D / 8)) * kPromptRows + tile * 128 + r;
 #pragma unroll
-        for (int i = 0; i < D; i += 32) {
-          uint32_t o[32];
-          tmem_ld32(tO + i, o);
-          tmem_wait_ld();
+        for (int i = 0; i < D / 2; i += 16) {
+          float o[16];
+          tmem_ld16(tO + i, o);
 #pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            pp[(i + k) / 4 * kPromptRows] = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]),
-                                                        __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+          for (int k = 0; k < 16; k += 4)
+            pp[(i + k) / 4 * kPromptRows] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
-        *reinterpret_cast<float2*>(p.a.ml + (slot * kPromptRows + tile * 128 + r) * 2) = make_float2(m, l);
+        if (half == 0) *reinterpret_cast<float2*>(p.a.ml + (slot * kPromptRows + tile * 128 + r) * 2) = make_float2(m, l);
       }
       tmem_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free + tile);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8 && lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kMma) {
       // ------------------------------ MMA issue ------------------------------
       // A and B bf16 (formats 1), D fp32; M = 128
       const uint32_t iS = umma_idesc_bf16(128), iO = umma_idesc_bf16(D) | (1u << 16);  // B of P V is N-major
-      uint32_t pq = 0, pfix = 0, pp[2] = {0, 0}, pof[2] = {1, 1};
+      const bool lead = elect_one();
+      const uint32_t q0 = (smem_u32(Qs) >> 4) | kDescQK, k0 = (smem_u32(KV) >> 4);
+      uint32_t pq = 0, pfix = 0, pp = 0, pof = 3;  // parities; pp, pof: a bit per tile
       int st = 0;
       uint32_t pst = 0;  // ring stage and parity of kv_full
-      const uint32_t qa = smem_u32(Qs), ka = smem_u32(KV);
       auto mma_s = [&](int tile, int stage) {
+        const uint32_t a = q0 + tile * (TILE >> 4), b = (k0 + stage * (TILE >> 4)) | kDescQK;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_ss(tmem + tile * 128, umma_desc_sw128(qa + tile * TILE + (k >> 2) * 16384 + (k & 3) * 32),
-                  umma_desc_sw128(ka + stage * TILE + (k >> 2) * 16384 + (k & 3) * 32), iS, k > 0);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+          umma_ss(tmem + tile * 128, a + off, b + off, iS, k > 0);
+        }
       };
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, unsigned code) {
-        ok = ok && prompt_wait(bar, parity, err, code);
+        ok = ok && prompt_warp_wait(bar, parity, err, code);
         return ok;
-      };
-      auto step = [&](int& s, uint32_t& par) {
-        if (++s == NS) { s = 0; par ^= 1; }
       };
       for (w.begin(p); ok && w.live(); w.next(p)) {
         const int tiles = w.second(p) ? 2 : 1, n = w.b1 - w.b0;
         if (!wait(q_full, pq, 0x47u) || !wait(kv_full + st, pst, 0x48u)) break;
         pq ^= 1;
         tmem_fence_after();
-        for (int i = 0; i < tiles; ++i) {
-          mma_s(i, st);
-          umma_commit(s_full + i);
+        if (lead) {
+          for (int i = 0; i < tiles; ++i) {
+            mma_s(i, st);
+            umma_commit(s_full + i);
+          }
+          umma_commit(kv_free + st);
+          if (n == 1) umma_commit(q_free);
         }
-        umma_commit(kv_free + st);
-        step(st, pst);
-        if (n == 1) umma_commit(q_free);
-        for (int j = 0; j < n && ok; ++j) {
+        __syncwarp();
+        if (++st == NS) { st = 0; pst ^= 1; }
+        for (int j = 0; j < n; ++j) {
           // stages: V(j) at st, K(j+1) after it
-          const int sv = st;
-          int sk = st;
-          uint32_t pk = pst;
-          step(sk, pk);
+          const bool more = j + 1 < n;
+          const int sv = st, sk = st + 1 == NS ? 0 : st + 1;
+          const uint32_t pk = st + 1 == NS ? pst ^ 1 : pst;
           if (!wait(kv_full + sv, pst, 0x48u)) break;
-          const bool tail = ((w.z.kb + w.b0 + j + 1) << 7) > w.z.len;
-          if (tail) {
+          if (((w.z.kb + w.b0 + j + 1) << 7) > w.z.len) {
             if (!wait(vfix, pfix, 0x49u)) break;
             pfix ^= 1;
           }
-          if (j + 1 < n && !wait(kv_full + sk, pk, 0x48u)) break;
+          if (more && !wait(kv_full + sk, pk, 0x48u)) break;
           for (int i = 0; i < tiles; ++i) {
-            if (!wait(p_ready + i, pp[i], 0x4Au)) break;
-            pp[i] ^= 1;
-            if (j == 0) {  // O of the previous item has been read
-              if (!wait(o_free + i, pof[i], 0x4Bu)) break;
-              pof[i] ^= 1;
-            }
+            if (!wait(p_ready + i, (pp >> i) & 1, 0x4Au)) break;
+            // O of the previous item has been read
+            if (j == 0 && !wait(o_free + i, (pof >> i) & 1, 0x4Bu)) break;
             tmem_fence_after();
+            if (lead) {
+              const uint32_t b = (k0 + sv * (TILE >> 4)) | kDescV;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_ts_bf16(tmem + 256 + i * D, tmem + i * 128 + k * 8, umma_desc_v(ka + sv * TILE + k * 2048), iO,
-                           j > 0 || k > 0);
-            if (j + 1 < n) {
-              mma_s(i, sk);
-              umma_commit(s_full + i);
-            } else {
-              umma_commit(o_full + i);
+              for (int k = 0; k < 8; ++k)
+                umma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, b + k * (2048 >> 4), iO, j > 0 || k > 0);
+              if (more) {
+                mma_s(i, sk);
+                umma_commit(s_full + i);
+              } else {
+                umma_commit(o_full + i);
+              }
             }
+            __syncwarp();
           }
           if (!ok) break;
-          umma_commit(kv_free + sv);
-          step(st, pst);
-          if (j + 1 < n) {
-            umma_commit(kv_free + sk);
-            step(st, pst);
+          pp ^= tiles == 2 ? 3u : 1u;
+          if (lead) {
+            umma_commit(kv_free + sv);
+            if (more) umma_commit(kv_free + sk);
+            if (j + 2 == n) umma_commit(q_free);  // the last S is issued
           }
-          if (j + 2 == n) umma_commit(q_free);  // the last S is issued
+          __syncwarp();
+          st = more ? (sk + 1 == NS ? 0 : sk + 1) : sk;
+          pst = st <= sv ? pst ^ 1 : pst;
         }
+        pof ^= tiles == 2 ? 3u : 1u;
       }
       if (!ok) {  // a wait gave up: let the issued MMAs finish before the memory goes
-        umma_commit(drain);
+        if (lead) umma_commit(drain);
+        __syncwarp();
         prompt_wait(drain, 0, err, 0x4Eu);
       }
-    } else if (warp == 9) {
+    } else if (warp == kMma + 1) {
       // -------------------------------- loads --------------------------------
       const int P = p.a.kv.P, rows = min(P, 128), nbox = 128 / rows;
       const int qbytes = p.TT * p.a.G * 128 * NH;
@@ -573,7 +685,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int k = max(0, issued - NS); k < issued; ++k)
         prompt_wait(kv_full + k % NS, (uint32_t)((k / NS) & 1), err, 0x4Eu);
       if (started) prompt_wait(q_full, pq, err, 0x4Eu);
-    } else if (warp == 10) {
+    } else if (warp == kMma + 2) {
       // ------------------ V rows past the sequence's end := 0 ------------------
       int st = 0;
       uint32_t pst = 0;
@@ -606,7 +718,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  if (warp == 8)
+  if (warp == kMma)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 

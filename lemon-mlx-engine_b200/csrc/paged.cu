@@ -327,6 +327,7 @@ int launch_prompt(const PagedAttnArgs& a, const AttnPlan& pl, cudaStream_t st) {
   PromptArgs p;
   p.a = a;
   p.TT = 128 / a.G;
+  p.cost = PromptSmem<D>::COST;
   p.start = (int4*)((uint8_t*)a.prefix + pl.start);
   PromptMaps mp;
   const cuuint64_t qd[3] = {D, (cuuint64_t)a.heads, (cuuint64_t)a.b.tokens};

@@ -27,7 +27,8 @@
 // bf16, whose exponents have room), so most tiles touch O in the MMA alone.
 //
 // Work split: as in the few-row kernel, the 128-key blocks of all items are
-// laid end to end and divided evenly over one CTA per SM; items that cross a
+// laid end to end, each item with a fixed cost of its own in front, and divided
+// evenly over one CTA per SM; items that cross a
 // boundary leave fp32 partials that paged_prompt_join_kernel adds in order.
 // The division is computed once, by paged_prompt_plan_kernel.
 #pragma once
@@ -43,7 +44,8 @@ static constexpr int kPromptRows = 256;  // rows of a pair
 struct PromptArgs {
   PagedAttnArgs a;   // nctas = CTAs of the grid; prefix[0] = total blocks; ml / part per slot of 256 rows
   int TT;            // tokens of one row tile
-  int4* start;       // [nctas] sequence, head, pair, block where a CTA begins
+  int cost;          // what an item costs beside its blocks, in blocks (PromptSmem)
+  int4* start;       // [nctas] where a CTA begins: sequence, head, pair, offset into the item
 };
 struct PromptMaps {
   CUtensorMap q, k, v;
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
     int64_t n = 0;
     for (int i = lane; i < z.pairs; i += 32) {
       prompt_pair(p, i, z);
-      n += z.nblk;
+      n += z.nblk + p.cost;
     }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
       int nb = 0;
       if (base + lane < z.pairs) {
         prompt_pair(p, base + lane, z);
-        nb = z.nblk;
+        nb = z.nblk + p.cost;
       }
       int inc = nb;
 #pragma unroll
@@ -154,41 +156,51 @@ __global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
   }
 }
 
-// A CTA's walk over its blocks: one segment (item, blocks [b0, b1)) at a time.
+// A CTA's walk over its share: one segment (item, blocks [b0, b1)) at a time.
+// A share that begins in an item's cost begins with its first block; one that
+// ends there has none of its blocks.
 struct PromptWalk {
   int seq, h, pair, b0, b1;
-  int64_t left;  // blocks from b0 to the CTA's end
+  int64_t left;  // of the share, from this segment on
+  int len;       // of this segment
   PromptItem z;
-  bool first;
+  bool first;    // the share begins with this item
 
+  LMX_DEV void cut(const PromptArgs& p, int off) {  // the segment that begins `off` into the item
+    len = (int)min((int64_t)(z.nblk + p.cost - off), left);
+    b0 = max(0, off - p.cost);
+    b1 = max(0, off + len - p.cost);
+  }
   LMX_DEV void begin(const PromptArgs& p) {
     const int64_t total = p.a.prefix[0], n = total < p.a.nctas ? total : p.a.nctas;
     left = 0;
     if (blockIdx.x >= n) return;
     left = total * (blockIdx.x + 1) / n - total * blockIdx.x / n;
     const int4 s = p.start[blockIdx.x];
-    seq = s.x; h = s.y; pair = s.z; b0 = s.w;
+    seq = s.x; h = s.y; pair = s.z;
     prompt_seq(p, seq, z);
     prompt_pair(p, pair, z);
-    b1 = (int)min((int64_t)z.nblk, b0 + left);
+    cut(p, s.w);
     first = true;
+    if (b1 == b0) next(p);
   }
   LMX_DEV bool live() const { return left > 0; }
   LMX_DEV void next(const PromptArgs& p) {
-    left -= b1 - b0;
-    first = false;
-    if (left <= 0) return;
-    b0 = 0;
-    if (++pair == z.pairs) {
-      pair = 0;
-      if (++h == p.a.kv.Hk) {
-        h = 0;
-        do prompt_seq(p, ++seq, z);
-        while (z.nnew == 0);
+    do {
+      left -= len;
+      first = false;
+      if (left <= 0) return;
+      if (++pair == z.pairs) {
+        pair = 0;
+        if (++h == p.a.kv.Hk) {
+          h = 0;
+          do prompt_seq(p, ++seq, z);
+          while (z.nnew == 0);
+        }
       }
-    }
-    prompt_pair(p, pair, z);
-    b1 = (int)min((int64_t)z.nblk, left);
+      prompt_pair(p, pair, z);
+      cut(p, 0);
+    } while (b1 == b0);
   }
   LMX_DEV bool second(const PromptArgs& p) const { return z.tn > p.TT; }  // the pair's second tile has rows
   LMX_DEV bool whole() const { return b0 == 0 && b1 == z.nblk; }
@@ -303,23 +315,28 @@ LMX_DEV void prompt_mask(uint32_t* s, int key, int klo, int khi) {
   for (int i = 0; i < 64; ++i)
     if (key + i >= khi || key + i < klo) s[i] = 0xff800000u;
 }
-LMX_DEV float prompt_max(const uint32_t* s) {  // of 64, in eight chains
+LMX_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+LMX_DEV float prompt_max(const uint32_t* s) {  // of 64, in eight chains; NaN if one is
   float m[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) m[k] = __uint_as_float(s[k]);
 #pragma unroll
   for (int i = 8; i < 56; i += 16)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m[k] = fmaxf(fmaxf(m[k], __uint_as_float(s[i + k])), __uint_as_float(s[i + 8 + k]));
+    for (int k = 0; k < 8; ++k) m[k] = max_nan(max_nan(m[k], __uint_as_float(s[i + k])), __uint_as_float(s[i + 8 + k]));
 #pragma unroll
-  for (int k = 0; k < 8; ++k) m[k] = fmaxf(m[k], __uint_as_float(s[56 + k]));
-  return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+  for (int k = 0; k < 8; ++k) m[k] = max_nan(m[k], __uint_as_float(s[56 + k]));
+  return max_nan(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])), max_nan(max_nan(m[4], m[5]), max_nan(m[6], m[7])));
 }
 // 2^x of a pair, x <= 2^8, on the FMA pipe: x = n + f, n the nearest integer
 // (the low bits of x + 1.5 * 2^23), 2^f by a degree-4 polynomial (least
 // maximal relative error over [-1/2, 1/2], 2.6e-6), n added to the exponent.
-// Below 2^-126 it stays there: only rows that see the whole tile come here, so
-// their sum is at least 2^-8.
+// Below 2^-126, masked scores included, it stays there, which is nothing beside
+// a row's largest p (at least 2^-8).
 LMX_DEV void ex2_pair(uint64_t x, float& p0, float& p1) {
   float x0, x1;
   f2_unpack(x, x0, x1);
@@ -338,10 +355,11 @@ LMX_DEV void ex2_pair(uint64_t x, float& p0, float& p1) {
   p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
   p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
 }
-#ifndef EMU
-#define EMU 0
-#endif
-// p = 2^(s * scale2 + ms) of 64 scores, stored as bf16 pairs; returns their sum.
+// p = 2^(s * scale2 + ms) of 64 scores, stored as bf16 pairs; returns their
+// sum.  Of eight pairs kPromptFma go to the FMA pipe: the special-function unit
+// alone would take as long as the MMAs (D = 128) or twice that (D = 64; ragged
+// 64-wide prompts 268 us with 0, 248 with 2, 278 with 4; D = 128 the same with 0 and 2).
+static constexpr int kPromptFma = 2;
 LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP) {
   const uint64_t sc = f2_pack(scale2, scale2), mm = f2_pack(ms, ms);
   uint64_t sum[4] = {};
@@ -352,7 +370,7 @@ LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP)
     for (int i = 0; i < 16; ++i) {
       const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[32 * h + 2 * i]), __uint_as_float(s[32 * h + 2 * i + 1])), sc, mm);
       float p0, p1;
-      if (i % 8 >= 8 - EMU) {
+      if (i % 8 >= 8 - kPromptFma) {
         ex2_pair(x, p0, p1);
       } else {
         f2_unpack(x, p0, p1);
@@ -378,6 +396,10 @@ template <int D>
 struct PromptSmem {
   static constexpr int TILE = 128 * D * 2;            // one tile of Q, K or V
   static constexpr int NS = D == 128 ? 5 : 8;         // K / V stages
+  // An item's own cost: its first scores and its last P V and output are not
+  // overlapped.  Without it the CTAs that get a prompt's short first items take
+  // 27% longer than the others (8192 tokens, 64 heads); swept 0 to 4 blocks.
+  static constexpr int COST = D == 128 ? 4 : 2;
   static constexpr int BYTES = 2 * TILE + NS * TILE + 256 + 2048;  // tiles, barriers, exchange
 };
 
@@ -477,7 +499,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tmem_fence_before();
         prompt_meet(tile);
         tmem_fence_after();
-        const float mx = fmaxf(mh, *other) * scale2;
+        const float mx = max_nan(mh, *other) * scale2;
+        if (mx != mx) l = mx;  // a NaN score shows in the row (the FMA-pipe exponentials would lose it)
         if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
           const float mn = fmaxf(m, mx);
           if (b > w.b0) {
@@ -511,6 +534,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         prompt_meet(tile);
       }
       po ^= 1;
+      if (m == -INFINITY && l == l) l = 0.0f;  // the row saw nothing
       tmem_fence_after();
       const int head = w.h * G + r % G;
       if (w.whole()) {
@@ -734,13 +758,13 @@ __global__ void __launch_bounds__(128) paged_prompt_join_kernel(const __grid_con
   const int64_t c = blockIdx.x;
   if (c >= n || c == 0) return;
   const int4 s = p.start[c];
-  if (s.w == 0) return;                             // begins with its item
-  const int64_t i0 = total * c / n - s.w;           // the item's first block
-  if (total * (c - 1) / n > i0) return;             // CTA c - 1 begins inside it too
+  if (s.w <= p.cost) return;               // begins with its item
+  const int64_t i0 = total * c / n - s.w;           // where the item begins
+  if (total * (c - 1) / n - i0 > p.cost) return;  // CTA c - 1 begins inside it too
   PromptItem z;
   prompt_seq(p, s.x, z);
   prompt_pair(p, s.z, z);
-  const int64_t c1 = ((i0 + z.nblk) * n - 1) / total;  // CTA of its last block
+  const int64_t c1 = ((i0 + p.cost + z.nblk) * n - 1) / total;  // CTA of its last block
   const int row = blockIdx.y * 32 + (threadIdx.x & 31), tile = row >> 7, r = row & 127;
   const int t = r / p.a.G, tok = z.t0 + tile * p.TT + t;
   if (t >= p.TT || tok >= z.nnew) return;

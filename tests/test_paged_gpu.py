@@ -374,6 +374,21 @@ def test_attention_prompt_kernel_large_scores(lmx, cuda, prompt_rows):
     check(cache, q, got, lse, 0.25, 0, p_err=2.0 ** -8)
 
 
+@pytest.mark.parametrize("rows", [1, 0])
+def test_attention_nan_stays_in_its_rows(lmx, cuda, prompt_rows, rows):
+    # a NaN query makes its own rows NaN and no others; a NaN key, every row that sees it
+    prompt_rows(rows)
+    cache = P.Cache(23, [(2, 300), (140, 140)], 1, 128, 16, 32)
+    cache.pool["k"][cache.at(0, torch.tensor([117]))] = math.nan
+    q = torch.randn((142, 2, 128), generator=cache.gen).to(BF16)
+    q[10, 1, 5] = math.nan
+    got, lse = attend(lmx, cache, q, 2, 0.1, 0)
+    bad = torch.zeros(142, 2, dtype=torch.bool)
+    bad[:2], bad[10, 1] = True, True
+    assert torch.equal(torch.isnan(got).all(-1), bad) and torch.equal(torch.isnan(got).any(-1), bad)
+    assert torch.equal(torch.isnan(lse), bad)
+
+
 def test_attention_peaked_and_large_scores(lmx, cuda):
     # one key takes all the weight, and scores far apart (hundreds in the exponent)
     cache = P.Cache(12, [(1, 333), (2, 64)], 2, 128, 16, 32, k_std=8.0)

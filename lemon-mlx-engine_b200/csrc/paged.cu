@@ -276,7 +276,7 @@ int check_attn(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads, 
     return set_error(LMX_ERR_UNSUPPORTED, "paged_attention: heads=%d over kv_heads=%d (a multiple, at most 64 times)",
                      heads, kv->kv_heads);
   const int D = kv->head_dim;
-  p.prompt = kv->bits == 16 && g_prompt_min_rows > 0 &&
+  p.prompt = g_prompt_min_rows > 0 &&
              (int64_t)batch->max_new * (heads / kv->kv_heads) >= g_prompt_min_rows;
   int rows = 16;  // of a partial result
   if (p.prompt) {
@@ -306,53 +306,53 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
-// bf16 map of `rank` dimensions, 128-byte swizzle, boxes of 64 values in the
-// first; strides in values
-int tensor_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides,
+// Map of `rank` dimensions: bf16 with the 128-byte swizzle (boxes of 64 values
+// in the first dimension), or 32-bit words as they are; strides in bytes.
+int tensor_map(CUtensorMap* m, const void* base, bool words, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                const cuuint32_t* box) {
   const auto encode = tensor_map_encoder();
   if (!encode) return set_error(LMX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  cuuint64_t st[3];
-  for (int i = 0; i + 1 < rank; ++i) st[i] = (cuuint64_t)strides[i] * 2;
   const cuuint32_t one[4] = {1, 1, 1, 1};
-  const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, st, box, one,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode(m, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                            const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            words ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(LMX_ERR_INVALID, "paged_attention: tensor map encode failed (%d)", (int)r);
   return LMX_OK;
 }
 
-template <int D>
+template <int D, int BITS>
 int launch_prompt(const PagedAttnArgs& a, const AttnPlan& pl, cudaStream_t st) {
   PromptArgs p;
   p.a = a;
   p.TT = 128 / a.G;
-  p.cost = PromptSmem<D>::COST;
+  p.cost = PromptSmem<D, BITS>::COST;
   p.start = (int4*)((uint8_t*)a.prefix + pl.start);
   PromptMaps mp;
   const cuuint64_t qd[3] = {D, (cuuint64_t)a.heads, (cuuint64_t)a.b.tokens};
-  const int64_t qs[2] = {D, a.ldq};
+  const cuuint64_t qs[2] = {D * 2, (cuuint64_t)a.ldq * 2};
   const cuuint32_t qb[3] = {64, (cuuint32_t)a.G, (cuuint32_t)p.TT};
-  int rc = tensor_map(&mp.q, a.q, 3, qd, qs, qb);
-  const cuuint64_t kd[4] = {D, (cuuint64_t)a.kv.P, (cuuint64_t)a.kv.Hk, (cuuint64_t)a.kv.pages};
-  const int64_t ks[3] = {D, (int64_t)a.kv.P * D, a.kv.pstride * D};
-  const cuuint32_t kb[4] = {64, (cuuint32_t)(a.kv.P < 128 ? a.kv.P : 128), 1, 1};
-  if (!rc) rc = tensor_map(&mp.k, a.kv.k, 4, kd, ks, kb);
-  if (!rc) rc = tensor_map(&mp.v, a.kv.v, 4, kd, ks, kb);
+  int rc = tensor_map(&mp.q, a.q, false, 3, qd, qs, qb);
+  constexpr cuuint64_t row = D * BITS / 8;  // bytes
+  const cuuint64_t kd[4] = {BITS == 16 ? D : row / 4, (cuuint64_t)a.kv.P, (cuuint64_t)a.kv.Hk, (cuuint64_t)a.kv.pages};
+  const cuuint64_t ks[3] = {row, (cuuint64_t)a.kv.P * row, (cuuint64_t)a.kv.pstride * row};
+  const cuuint32_t kb[4] = {BITS == 16 ? 64 : (cuuint32_t)row / 4, (cuuint32_t)(a.kv.P < 128 ? a.kv.P : 128), 1, 1};
+  if (!rc) rc = tensor_map(&mp.k, a.kv.k, BITS != 16, 4, kd, ks, kb);
+  if (!rc) rc = tensor_map(&mp.v, a.kv.v, BITS != 16, 4, kd, ks, kb);
   if (rc) return rc;
   static bool attr_set[64] = {};
   int d = 0;
   cudaGetDevice(&d);
-  constexpr int smem = PromptSmem<D>::BYTES;
+  constexpr int smem = PromptSmem<D, BITS>::BYTES;
   if (!attr_set[d & 63]) {
-    rc = cuda_check(cudaFuncSetAttribute(paged_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+    rc = cuda_check(cudaFuncSetAttribute(paged_prompt_kernel<D, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                     "paged_attention: set smem");
     if (rc) return rc;
     attr_set[d & 63] = true;
   }
   rc = cuda_check(lmx_launch(paged_prompt_plan_kernel, dim3(1), dim3(1024), 0, st, true, p), "paged_attention: plan launch");
   if (!rc)
-    rc = cuda_check(lmx_launch(paged_prompt_kernel<D>, dim3(a.nctas), dim3(kPromptThreads), smem, st, true, mp, p),
+    rc = cuda_check(lmx_launch(paged_prompt_kernel<D, BITS>, dim3(a.nctas), dim3(prompt_threads(BITS)), smem, st, true, mp, p),
                     "paged_attention: prompt launch");
   if (!rc)
     rc = cuda_check(lmx_launch(paged_prompt_join_kernel<D>, dim3(a.nctas, kPromptRows / 32), dim3(128), 0, st, true, p),
@@ -420,7 +420,11 @@ extern "C" int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch
   a.nctas = p.nctas;
   a.err = device_error_word();
   cudaStream_t st = (cudaStream_t)stream;
-  if (p.prompt) return D == 64 ? launch_prompt<64>(a, p, st) : launch_prompt<128>(a, p, st);
+  if (p.prompt) {
+    if (D == 64)
+      return kv->bits == 16 ? launch_prompt<64, 16>(a, p, st) : kv->bits == 8 ? launch_prompt<64, 8>(a, p, st) : launch_prompt<64, 4>(a, p, st);
+    return kv->bits == 16 ? launch_prompt<128, 16>(a, p, st) : kv->bits == 8 ? launch_prompt<128, 8>(a, p, st) : launch_prompt<128, 4>(a, p, st);
+  }
   if (D == 64)
     return kv->bits == 16 ? launch_few<64, 16>(a, st) : kv->bits == 8 ? launch_few<64, 8>(a, st) : launch_few<64, 4>(a, st);
   return kv->bits == 16 ? launch_few<128, 16>(a, st) : kv->bits == 8 ? launch_few<128, 8>(a, st) : launch_few<128, 4>(a, st);

@@ -38,7 +38,9 @@
 namespace lmx {
 
 static constexpr int kPromptSoftmaxWarps = 16;  // per row tile: two halves of four
-static constexpr int kPromptThreads = 32 * kPromptSoftmaxWarps + 128;
+// + MMA, loads, V clearing (idle for quantized caches) and one spare; + four
+// warps that dequantize
+constexpr int prompt_threads(int bits) { return 32 * kPromptSoftmaxWarps + (bits == 16 ? 128 : 256); }
 static constexpr int kPromptRows = 256;  // rows of a pair
 
 struct PromptArgs {
@@ -355,11 +357,12 @@ LMX_DEV void ex2_pair(uint64_t x, float& p0, float& p1) {
   p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
   p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
 }
-// p = 2^(s * scale2 + ms) of 64 scores, stored as bf16 pairs; returns their
-// sum.  Of eight pairs kPromptFma go to the FMA pipe: the special-function unit
+// p = 2^(s * scale2 + ms) of 64 scores, stored as pairs (bf16; fp16
+// for quantized caches); returns their sum.  Of eight pairs kPromptFma go to the FMA pipe: the special-function unit
 // alone would take as long as the MMAs (D = 128) or twice that (D = 64; ragged
 // 64-wide prompts 268 us with 0, 248 with 2, 278 with 4; D = 128 the same with 0 and 2).
 static constexpr int kPromptFma = 2;
+template <int BITS>
 LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP) {
   const uint64_t sc = f2_pack(scale2, scale2), mm = f2_pack(ms, ms);
   uint64_t sum[4] = {};
@@ -378,7 +381,8 @@ LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP)
         p1 = ex2f(p1);
       }
       sum[i & 3] = f2_add(sum[i & 3], f2_pack(p0, p1));
-      pk[i] = pk_bf2(p0, p1);
+      if (BITS == 16) pk[i] = pk_bf2(p0, p1);
+      else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[i]) : "f"(p1), "f"(p0));
     }
     tmem_st16(tP + 16 * h, pk);
   }
@@ -392,21 +396,96 @@ LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP)
 // the leading offset goes from one 64-value block to the next, 128 keys * 128 B.
 static constexpr uint32_t kDescQK = 1u << 16, kDescV = (16384u >> 4) << 16;
 
-template <int D>
+template <int D, int BITS>
 struct PromptSmem {
-  static constexpr int TILE = 128 * D * 2;            // one tile of Q, K or V
-  static constexpr int NS = D == 128 ? 5 : 8;         // K / V stages
+  static constexpr int TILE = 128 * D * 2;            // one tile of Q, K or V, 16-bit
+  static constexpr int RAW = BITS == 16 ? 0 : 128 * D * BITS / 8;  // a packed tile of K or V
+  static constexpr int NR = BITS == 16 ? 1 : D * BITS >= 1024 ? 2 : 4;  // packed stages
+  static constexpr int NS = D == 128 ? (BITS == 16 ? 5 : 4) : 8;   // K / V stages
   // An item's own cost: its first scores and its last P V and output are not
   // overlapped.  Without it the CTAs that get a prompt's short first items take
   // 27% longer than the others (8192 tokens, 64 heads); swept 0 to 4 blocks.
   static constexpr int COST = D == 128 ? 4 : 2;
-  static constexpr int BYTES = 2 * TILE + NS * TILE + 256 + 2048;  // tiles, barriers, exchange
+  static constexpr int BARS = (12 + 2 * NS + 2 * NR + 1) * 8 + 8;
+  static constexpr int XCH = (BARS + 127) / 128 * 128;
+  static constexpr int BYTES = 2 * TILE + NS * TILE + NR * RAW + XCH + 2048;  // tiles, barriers, exchange
 };
 
-template <int D>
-__global__ void __launch_bounds__(kPromptThreads, 1)
+// ---- quantized caches: 16 codes -> 16 fp16 values, fma(code, scale, bias) ----
+// fp16 because its 11 bits lose nothing that matters to bf16 outputs, where
+// bf16 values would add two roundings of the outputs' own size; scale, bias and
+// values saturate at 65504.  Codes become 1024 + code by giving a half the
+// exponent of 1024; subtracting 1024 is exact and the fma rounds once.
+LMX_DEV uint32_t h2_sat(float v) {  // both halves
+  uint32_t r;
+  const float c = fminf(fmaxf(v, -65504.0f), 65504.0f);
+  asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(r) : "f"(c));
+  return r;
+}
+LMX_DEV uint32_t h2_deq(uint32_t x, uint32_t s, uint32_t b) {
+  uint32_t c, v;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(c) : "r"(x), "r"(0xE400E400u));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(c), "r"(s), "r"(b));
+  return v;
+}
+template <int BITS>
+LMX_DEV void prompt_deq16(const uint8_t* raw, uint32_t s, uint32_t b, uint4& lo, uint4& hi) {
+  uint32_t o[8];
+  if constexpr (BITS == 8) {
+    const uint4 w = *reinterpret_cast<const uint4*>(raw);
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[2 * i] = h2_deq(__byte_perm(ws[i], 0x64646464u, 0x4140), s, b);
+      o[2 * i + 1] = h2_deq(__byte_perm(ws[i], 0x64646464u, 0x4342), s, b);
+    }
+  } else {  // the eight values of a word come out in the order 0 4 1 5 2 6 3 7
+    const uint2 w = *reinterpret_cast<const uint2*>(raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = h2_deq(((w.x >> (4 * i)) & 0x000F000Fu) | 0x64006400u, s, b);
+      o[4 + i] = h2_deq(((w.y >> (4 * i)) & 0x000F000Fu) | 0x64006400u, s, b);
+    }
+  }
+  lo = make_uint4(o[0], o[1], o[2], o[3]);
+  hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+// eight bf16 query values -> fp16, in the order of the keys' values
+template <int BITS>
+LMX_DEV uint4 prompt_q8(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = fminf(fmaxf(lo_bf(w[i]), -65504.0f), 65504.0f), b = fminf(fmaxf(hi_bf(w[i]), -65504.0f), 65504.0f);
+    const float x = lo_bf(w[i]) != lo_bf(w[i]) ? lo_bf(w[i]) : a, y = hi_bf(w[i]) != hi_bf(w[i]) ? hi_bf(w[i]) : b;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(y), "f"(x));
+  }
+  if (BITS == 8) return make_uint4(h[0], h[1], h[2], h[3]);
+  return make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410),
+                    __byte_perm(h[1], h[3], 0x7632));
+}
+// the output columns back in order
+template <int BITS>
+LMX_DEV void prompt_order(float* y) {
+  if (BITS != 4) return;
+#pragma unroll
+  for (int k = 0; k < 16; k += 8) {
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = y[k + i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[k + i] = t[2 * i];
+      y[k + i + 4] = t[2 * i + 1];
+    }
+  }
+}
+
+template <int D, int BITS>
+__global__ void __launch_bounds__(prompt_threads(BITS), 1)
     paged_prompt_kernel(const __grid_constant__ PromptMaps mp, const __grid_constant__ PromptArgs p) {
-  using SM = PromptSmem<D>;
+  using SM = PromptSmem<D, BITS>;
   constexpr int TILE = SM::TILE, NS = SM::NS, NH = D / 64, kMma = kPromptSoftmaxWarps;
   // the tiles' swizzle wants 1024-byte alignment: the kernel has no static
   // shared memory, so the dynamic part begins at a multiple of 1024 (checked)
@@ -417,15 +496,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   }
   uint8_t* Qs = smem;
   uint8_t* KV = smem + 2 * TILE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(KV + NS * TILE);
+  uint8_t* raw = KV + NS * TILE;
+  uint8_t* rest = raw + SM::NR * SM::RAW;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(rest);
   uint64_t *q_full = bars, *q_free = bars + 1, *vfix = bars + 2, *s_full = bars + 3, *p_ready = bars + 5,
            *o_full = bars + 7, *o_free = bars + 9, *drain = bars + 11, *kv_full = bars + 12, *kv_free = kv_full + NS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_free + NS);
-  float* xch = reinterpret_cast<float*>(KV + NS * TILE + 256);  // [tile][half][128]
+  uint64_t *q_raw = kv_free + NS, *raw_full = q_raw + 1, *raw_free = raw_full + SM::NR;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_free + SM::NR);
+  float* xch = reinterpret_cast<float*>(rest + SM::XCH);  // [tile][half][128]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
+    mbar_init(q_full, BITS == 16 ? 1 : 4);
+    mbar_init(q_raw, 1);
     mbar_init(q_free, 1);
     mbar_init(vfix, 1);
     mbar_init(drain, 1);
@@ -436,8 +519,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(o_free + i, 8);
     }
     for (int i = 0; i < NS; ++i) {
-      mbar_init(kv_full + i, 1);
-      mbar_init(kv_free + i, 2);  // the MMAs' commit and the warp that clears V
+      mbar_init(kv_full + i, BITS == 16 ? 1 : 4);
+      mbar_init(kv_free + i, BITS == 16 ? 2 : 1);  // the MMAs' commit and the warp that clears V
+    }
+    for (int i = 0; i < SM::NR; ++i) {
+      mbar_init(raw_full + i, 1);
+      mbar_init(raw_free + i, 4);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -457,7 +544,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   if (warp < kPromptSoftmaxWarps) {
     // ------------------------- softmax and epilogue -------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    if constexpr (BITS == 16) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
     const int tile = warp >> 3, half = (warp >> 2) & 1;  // of the pair; of the tile's columns
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's 32 TMEM lanes
     const uint32_t tS = tmem + lanes + tile * 128, tO = tmem + lanes + 256 + tile * D + half * (D / 2);
@@ -466,6 +554,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const float* other = xch + (tile * 2 + (half ^ 1)) * 128 + r;
     const int G = p.a.G;
     const float scale2 = p.a.scale2;
+    constexpr float kLift = BITS == 16 ? 0.0f : 7.0f;  // fp16 p: up to 2^15, so that small ones keep their bits
     uint32_t ps = 0, po = 0;  // parities of s_full, o_full
     bool ok = true;
     // A wait that gives up is the last one; the rest then runs through on
@@ -518,7 +607,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
           m = mn;
         }
-        l += prompt_exp(s, scale2, m == -INFINITY ? 0.0f : -m, tS + 32 * half);
+        l += prompt_exp<BITS>(s, scale2, m == -INFINITY ? 0.0f : kLift - m, tS + 32 * half);
         tmem_wait_st();
         tmem_fence_before();
         __syncwarp();
@@ -544,6 +633,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int i = 0; i < D / 2; i += 16) {
           float o[16];
           tmem_ld16(tO + i, o);
+          prompt_order<BITS>(o);
           if (row)
 #pragma unroll
             for (int k = 0; k < 16; k += 8) {
@@ -555,7 +645,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         if (half == 0 && row && p.a.lse)
           p.a.lse[(int64_t)(w.z.first + tok) * p.a.heads + head] =
-              l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+              l == 0.0f ? -INFINITY : (m - kLift + log2f(l)) * 0.693147180559945309f;
       } else {
         const int64_t slot = 2 * (int64_t)blockIdx.x + (w.first ? 0 : 1);
         float4* pp = reinterpret_cast<float4*>(p.a.part) + (slot * (D / 4) + half * (D / 8)) * kPromptRows + tile * 128 + r;
@@ -563,22 +653,114 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int i = 0; i < D / 2; i += 16) {
           float o[16];
           tmem_ld16(tO + i, o);
+          prompt_order<BITS>(o);
 #pragma unroll
           for (int k = 0; k < 16; k += 4)
             pp[(i + k) / 4 * kPromptRows] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
-        if (half == 0) *reinterpret_cast<float2*>(p.a.ml + (slot * kPromptRows + tile * 128 + r) * 2) = make_float2(m, l);
+        if (half == 0) *reinterpret_cast<float2*>(p.a.ml + (slot * kPromptRows + tile * 128 + r) * 2) = make_float2(m - kLift, l);
       }
       tmem_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free + tile);
     }
+  } else if (BITS != 16 && warp >= kMma + 4) {
+    // ----------------------------- dequantize -----------------------------
+    // A lane turns 16 codes of a row at a time; a warp owns 32 rows of each
+    // tile.  The scales of the next tile of the same kind are loaded before
+    // this one is converted.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (BITS != 16) {
+      constexpr int U = D / 16, RPI = 32 / U, IT = 32 / RPI, NG = D / 64;  // units per row, rows per pass, passes
+      const int dw = warp - kMma - 4, u = lane % U, r0 = dw * 32 + lane / U;
+      const PagedKv& kv = p.a.kv;
+      int st = 0, rs = 0;
+      uint32_t pst = 1, prs = 0, pq = 0;  // parities of kv_free, raw_full, q_raw
+      bool ok = true;
+      // rows of the head: the warp's first and second 16 keys of block b (-1: none)
+      auto rows_of = [&](int b, int64_t (&at)[2]) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int key = ((w.z.kb + b) << 7) + dw * 32 + 16 * k;
+          at[k] = -1;
+          if (b < w.b1 && key < w.z.hi && key + 16 > w.z.lo) {
+            const int64_t r = paged_row(kv, p.a.b, w.seq, key);
+            at[k] = r < 0 ? -1 : r + (int64_t)w.h * kv.P;
+          }
+        }
+      };
+      auto load_sb = [&](const bf16_t* sc, const bf16_t* bi, int b, const int64_t (&at)[2], uint32_t (&sb)[IT]) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          const int r = lane / U + RPI * i;  // of the warp's 32
+          sb[i] = 0;                         // rows that are not there read as zeros
+          const int64_t base = at[(RPI * i) >> 4];
+          if (base >= 0 && ((w.z.kb + b) << 7) + dw * 32 + r < w.z.len) {
+            const int64_t x = (base + (r & 15)) * NG + u / (U / NG);
+            sb[i] = (uint32_t)__ldg(sc + x) | ((uint32_t)__ldg(bi + x) << 16);
+          }
+        }
+      };
+      for (w.begin(p); ok && w.live(); w.next(p)) {
+        int64_t at[2];
+        uint32_t sk[IT], sv[IT];
+        rows_of(w.b0, at);
+        load_sb(kv.ks, kv.kb, w.b0, at, sk);
+        load_sb(kv.vs, kv.vb, w.b0, at, sv);
+        ok = prompt_warp_wait(q_raw, pq, err, 0x53u);
+        if (!ok) break;
+        pq ^= 1;
+        const int tiles = w.second(p) ? 2 : 1;
+        for (int i = threadIdx.x & 127; i < tiles * (TILE / 16); i += 128) {
+          uint4* q = reinterpret_cast<uint4*>(Qs) + i;
+          *q = prompt_q8<BITS>(*q);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        for (int b = w.b0; b < w.b1 && ok; ++b) {
+          rows_of(b + 1, at);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t(&sb)[IT] = h ? sv : sk;
+            ok = prompt_warp_wait(raw_full + rs, prs, err, 0x54u) && prompt_warp_wait(kv_free + st, pst, err, 0x55u);
+            if (!ok) break;
+            const uint8_t* src = raw + rs * SM::RAW + r0 * (D * BITS / 8) + u * (2 * BITS);
+            uint8_t* dst = KV + st * TILE;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+              const int r = r0 + RPI * i;
+              uint4 v[2];
+              prompt_deq16<BITS>(src + RPI * i * (D * BITS / 8), h2_sat(lo_bf(sb[i])), h2_sat(hi_bf(sb[i])), v[0], v[1]);
+              // 16-byte chunks 2u, 2u+1 of the row; lanes of the second 64 head
+              // dims take theirs in the other order, so that eight lanes write eight banks
+              const int c = (2 * u) & 7, sw = (u >> 2) & 1;
+              uint8_t* row = dst + (u >> 2) * 16384 + r * 128;
+              *reinterpret_cast<uint4*>(row + (((c + sw) ^ (r & 7)) << 4)) = sw ? v[1] : v[0];
+              *reinterpret_cast<uint4*>(row + (((c + 1 - sw) ^ (r & 7)) << 4)) = sw ? v[0] : v[1];
+            }
+            if (h == 0) load_sb(kv.ks, kv.kb, b + 1, at, sk);
+            else load_sb(kv.vs, kv.vb, b + 1, at, sv);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(kv_full + st);
+              mbar_arrive(raw_free + rs);
+            }
+            if (++st == NS) { st = 0; pst ^= 1; }
+            if (++rs == SM::NR) { rs = 0; prs ^= 1; }
+          }
+        }
+      }
+    }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (BITS == 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == kMma) {
       // ------------------------------ MMA issue ------------------------------
-      // A and B bf16 (formats 1), D fp32; M = 128
-      const uint32_t iS = umma_idesc_bf16(128), iO = umma_idesc_bf16(D) | (1u << 16);  // B of P V is N-major
+      // A and B bf16 (fp16 for quantized caches: formats 0), D fp32; M = 128
+      constexpr uint32_t kFormats = BITS == 16 ? 0 : (1u << 7) | (1u << 10);
+      const uint32_t iS = umma_idesc_bf16(128) ^ kFormats, iO = (umma_idesc_bf16(D) ^ kFormats) | (1u << 16);  // B of P V is N-major
       const bool lead = elect_one();
       const uint32_t q0 = (smem_u32(Qs) >> 4) | kDescQK, k0 = (smem_u32(KV) >> 4);
       uint32_t pq = 0, pfix = 0, pp = 0, pof = 3;  // parities; pp, pof: a bit per tile
@@ -618,7 +800,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const int sv = st, sk = st + 1 == NS ? 0 : st + 1;
           const uint32_t pk = st + 1 == NS ? pst ^ 1 : pst;
           if (!wait(kv_full + sv, pst, 0x48u)) break;
-          if (((w.z.kb + w.b0 + j + 1) << 7) > w.z.len) {
+          if (BITS == 16 && ((w.z.kb + w.b0 + j + 1) << 7) > w.z.len) {
             if (!wait(vfix, pfix, 0x49u)) break;
             pfix ^= 1;
           }
@@ -662,6 +844,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
     } else if (warp == kMma + 1) {
       // -------------------------------- loads --------------------------------
+      // bf16: K and V tiles straight into the MMAs' ring; quantized: packed tiles
+      // into theirs, Q for the dequantizing warps to convert in place
+      constexpr int N = BITS == 16 ? NS : SM::NR, BYTES = BITS == 16 ? TILE : SM::RAW, NB = BITS == 16 ? NH : 1;
+      uint8_t* ring = BITS == 16 ? KV : raw;
+      uint64_t *full = BITS == 16 ? kv_full : raw_full, *free_ = BITS == 16 ? kv_free : raw_free;
+      uint64_t* qbar = BITS == 16 ? q_full : q_raw;
       const int P = p.a.kv.P, rows = min(P, 128), nbox = 128 / rows;
       const int qbytes = p.TT * p.a.G * 128 * NH;
       int st = 0;
@@ -675,10 +863,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         pq ^= 1;
         started = true;
         if (lane == 0) {
-          mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * qbytes));
+          mbar_arrive_expect_tx(qbar, (uint32_t)(tiles * qbytes));
           for (int i = 0; i < tiles; ++i)
             for (int h = 0; h < NH; ++h)
-              tma_load_3d(Qs + i * TILE + h * 16384, &mp.q, h * 64, w.h * p.a.G, w.z.first + w.z.t0 + i * p.TT, q_full);
+              tma_load_3d(Qs + i * TILE + h * 16384, &mp.q, h * 64, w.h * p.a.G, w.z.first + w.z.t0 + i * p.TT, qbar);
         }
         for (int b = w.b0; b < w.b1 && ok; ++b) {
           const int key = (w.z.kb + b) * 128 + lane * rows;
@@ -692,24 +880,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            ok = prompt_warp_wait(kv_free + st, pst, err, 0x4Du);
+            ok = prompt_warp_wait(free_ + st, pst, err, 0x4Du);
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(kv_full + st, (uint32_t)TILE);
+            if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)BYTES);
             __syncwarp();
             if (lane < nbox)
-              for (int h = 0; h < NH; ++h)
-                tma_load_4d(KV + st * TILE + h * 16384 + lane * rows * 128, kv ? &mp.v : &mp.k, h * 64, key & (P - 1),
-                            w.h, page, kv_full + st);
+              for (int h = 0; h < NB; ++h)
+                tma_load_4d(ring + st * BYTES + h * 16384 + lane * rows * (BITS == 16 ? 128 : D * BITS / 8),
+                            kv ? &mp.v : &mp.k, h * 64, key & (P - 1), w.h, page, full + st);
             ++issued;
-            if (++st == NS) { st = 0; pst ^= 1; }
+            if (++st == N) { st = 0; pst ^= 1; }
           }
         }
       }
       // leave no copy in flight behind, also where a wait gave up
-      for (int k = max(0, issued - NS); k < issued; ++k)
-        prompt_wait(kv_full + k % NS, (uint32_t)((k / NS) & 1), err, 0x4Eu);
-      if (started) prompt_wait(q_full, pq, err, 0x4Eu);
-    } else if (warp == kMma + 2) {
+      for (int k = max(0, issued - N); k < issued; ++k)
+        prompt_wait(full + k % N, (uint32_t)((k / N) & 1), err, 0x4Eu);
+      if (started) prompt_wait(qbar, pq, err, 0x4Eu);
+    } else if (BITS == 16 && warp == kMma + 2) {
       // ------------------ V rows past the sequence's end := 0 ------------------
       int st = 0;
       uint32_t pst = 0;

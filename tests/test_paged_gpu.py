@@ -348,7 +348,7 @@ PROMPT = {"one": [(1, 1)], "prompt": [(200, 200)], "tile edges": [(128, 128), (1
 
 # rows at the 128-key tile's and the page's ends, every grouping (rows of a
 # tile that 128 / G does not fill), windows that end inside a tile and a page
-@pytest.mark.parametrize("bits", [16])
+@pytest.mark.parametrize("bits", [16, 8, 4])
 @pytest.mark.parametrize("lens,hk,g,d,page,window", [
     ("one", 1, 1, 128, 16, 0), ("prompt", 2, 1, 64, 32, 0), ("prompt", 1, 4, 128, 128, 0), ("tile edges", 2, 4, 128, 16, 0),
     ("tile edges", 1, 3, 64, 64, 50), ("tile edges", 1, 1, 128, 256, 128), ("ragged", 2, 4, 128, 32, 0),
@@ -362,8 +362,11 @@ def test_attention_prompt_kernel(lmx, cuda, prompt_rows, bits, lens, hk, g, d, p
     P.device_error(lmx)
     got, lse = attend(lmx, cache, q, hk * g, d ** -0.5, window, extra=8 if g == 2 else 0)
     assert P.device_error(lmx) == 0
-    # p enters P V as bf16: 2^-8
-    check(cache, q, got, lse, d ** -0.5, window, p_err=2.0 ** -8)
+    # p enters P V as bf16: 2^-8; over a quantized cache p and the K and V values are fp16: 2^-11
+    if bits == 16:
+        check(cache, q, got, lse, d ** -0.5, window, p_err=2.0 ** -8)
+    else:
+        check(cache, q, got, lse, d ** -0.5, window, p_err=2.0 ** -11, kv_err=2.0 ** -11)
 
 
 def test_attention_prompt_kernel_large_scores(lmx, cuda, prompt_rows):

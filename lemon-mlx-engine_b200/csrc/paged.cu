@@ -366,7 +366,7 @@ int launch_few(const PagedAttnArgs& a, cudaStream_t st) {
                       "paged_attention: launch");
   if (rc) return rc;
   unsigned grid;
-  if ((rc = grid_of(((int64_t)a.b.tokens * a.heads + 3) / 4, grid, "paged_attention"))) return rc;
+  if ((rc = grid_of((int64_t)a.b.tokens * a.heads, grid, "paged_attention"))) return rc;
   return cuda_check(lmx_launch(paged_combine_kernel<D>, dim3(grid), dim3(128), 0, st, true, a),
                     "paged_attention: join launch");
 }

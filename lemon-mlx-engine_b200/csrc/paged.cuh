@@ -49,6 +49,14 @@ LMX_DEV void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+LMX_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // The sequence that owns packed token t: how many of q_start[1..seqs] are
 // <= t.  The warp probes 32 entries at a time; sequences without new tokens
 // are passed over because their entries repeat.
@@ -446,9 +454,10 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
 //
 // Precision: scores and sums fp32; p enters P V as two bf16 terms
 // p_hi = bf16(p), p_lo = bf16(p - p_hi) (17 significant bits) because one term
-// would double the output's rounding error and the tensor pipe is idle enough
-// for both.  Quantized caches: codes enter the MMAs exactly and scale / bias are applied
-// outside, per group of 64 head dims,
+// would add an error of the output's own rounding and the tensor pipe is idle
+// enough for both.  Quantized caches: codes enter the MMAs exactly (as 1024 +
+// code in fp16 or 128 + code in bf16 against the queries; queries past fp16's
+// 65504 saturate) and scale / bias are applied outside, per group of 64 head dims,
 //   q.k = sum_g s_g (q_g . c_g) + b_g sum q_g,
 //   sum_j p_j v_j = sum_j (p_j s_j) (c_j - z) + sum_j p_j (b_j + z s_j),
 // z = 8 or 128 being the middle of the code range, so that the first sum
@@ -543,61 +552,75 @@ LMX_DEV void ld_words(uint32_t* d, const uint8_t* p) {
   }
 }
 
-// K fragments (and the quantizer's scales and biases) of the 16 keys whose
-// first row is `row`; keys past `n` are not read (their scores are masked).
-template <int D, int BITS>
-LMX_DEV void paged_load_k(PagedFrag<D, BITS>& f, const PagedKv& kv, int64_t row, int n, int g, int c) {
-  using F = PagedFrag<D, BITS>;
-  constexpr int RB = D * BITS / 8;               // bytes of a row
-  constexpr int CH = BITS == 16 ? 64 : 64 * BITS / 8;  // bytes of one chunk (32 values, or a group of 64)
+// scales or biases of keys 2c, 2c+1 (+ 8 kt) from `base`, row `row`; keys past n
+// get zeros, whatever the page holds there
+template <int NG, bool WHOLE>
+LMX_DEV void paged_load_sb(uint32_t (&d)[2][NG], const bf16_t* base, int64_t row, int n, int c) {
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    const bool there = row >= 0 && 8 * kt + g < n;
-    const uint8_t* p = kv.k + (row + 8 * kt + g) * RB + c * (CH / 4);
-#pragma unroll
-    for (int w = 0; w < F::KW; ++w) f.k[kt][w] = 0;
-    if (there) {
-#pragma unroll
-      for (int i = 0; i < RB / CH; ++i) ld_words<CH / 16>(f.k[kt] + i * (CH / 16), p + i * CH);
-    }
-    if constexpr (BITS != 16) {
-#pragma unroll
-      for (int w = 0; w < F::NG; ++w) f.ks[kt][w] = f.kb[kt][w] = 0;
-      if (row >= 0) {  // whole pages hold 16 scales: rows past n are within the page
-        const int64_t at = (row + 8 * kt + 2 * c) * F::NG;
-        ld_words<F::NG>(f.ks[kt], reinterpret_cast<const uint8_t*>(kv.ks + at));
-        ld_words<F::NG>(f.kb[kt], reinterpret_cast<const uint8_t*>(kv.kb + at));
+    const int key = 8 * kt + 2 * c;
+    ld_words<NG>(d[kt], reinterpret_cast<const uint8_t*>(base + (row + key) * NG));
+    if constexpr (!WHOLE) {
+      if constexpr (NG == 2) {
+        if (key >= n) d[kt][0] = 0;
+        if (key + 1 >= n) d[kt][1] = 0;
+      } else {
+        if (key >= n) d[kt][0] = 0;
+        if (key + 1 >= n) d[kt][0] &= 0xffffu;
       }
     }
   }
 }
-// V fragments: rows 2c, 2c+1, 2c+8, 2c+9; rows past n read as zero, whatever
-// the page holds there.
-template <int D, int BITS>
+// K fragments (and the quantizer's scales and biases) of the 16 keys whose
+// first row is `row`.  WHOLE: all 16 are there.  Else only the first n, and
+// none if row < 0 (no page): the others read as zeros.
+template <int D, int BITS, bool WHOLE>
+LMX_DEV void paged_load_k(PagedFrag<D, BITS>& f, const PagedKv& kv, int64_t row, int n, int g, int c) {
+  using F = PagedFrag<D, BITS>;
+  constexpr int RB = D * BITS / 8;               // bytes of a row
+  constexpr int CH = BITS == 16 ? 64 : 64 * BITS / 8;  // bytes of one chunk (32 values, or a group of 64)
+  if (!WHOLE && row < 0) {
+    row = 0;
+    n = 0;
+  }
+  const uint8_t* p = kv.k + (row + g) * RB + c * (CH / 4);
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    if (!WHOLE)
+#pragma unroll
+      for (int w = 0; w < F::KW; ++w) f.k[kt][w] = 0;
+    if (WHOLE || 8 * kt + g < n)
+#pragma unroll
+      for (int i = 0; i < RB / CH; ++i) ld_words<CH / 16>(f.k[kt] + i * (CH / 16), p + 8 * kt * RB + i * CH);
+  }
+  if constexpr (BITS != 16) {
+    paged_load_sb<F::NG, WHOLE>(f.ks, kv.ks, row, n, c);
+    paged_load_sb<F::NG, WHOLE>(f.kb, kv.kb, row, n, c);
+  }
+}
+// V fragments: rows 2c, 2c+1, 2c+8, 2c+9
+template <int D, int BITS, bool WHOLE>
 LMX_DEV void paged_load_v(PagedFrag<D, BITS>& f, const PagedKv& kv, int64_t row, int n, int g, int c) {
   using F = PagedFrag<D, BITS>;
   constexpr int RB = D * BITS / 8, CH = RB / (D / 64);  // bytes of 64 values
+  if (!WHOLE && row < 0) {
+    row = 0;
+    n = 0;
+  }
+  const uint8_t* p = kv.v + (row + 2 * c) * RB + g * (CH / 8);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int key = 2 * c + (r & 1) + 8 * (r >> 1);
-    const uint8_t* p = kv.v + (row + key) * RB + g * (CH / 8);
+    const int key = (r & 1) + 8 * (r >> 1);
+    if (!WHOLE)
 #pragma unroll
-    for (int w = 0; w < F::VW; ++w) f.v[r][w] = 0;
-    if (row >= 0 && key < n)
+      for (int w = 0; w < F::VW; ++w) f.v[r][w] = 0;
+    if (WHOLE || 2 * c + key < n)
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) ld_words<CH / 32>(f.v[r] + i * (CH / 32), p + i * CH);
+      for (int i = 0; i < D / 64; ++i) ld_words<CH / 32>(f.v[r] + i * (CH / 32), p + key * RB + i * CH);
   }
   if constexpr (BITS != 16) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-      for (int w = 0; w < F::NG; ++w) f.vs[kt][w] = f.vb[kt][w] = 0;
-      if (row >= 0) {
-        const int64_t at = (row + 8 * kt + 2 * c) * F::NG;
-        ld_words<F::NG>(f.vs[kt], reinterpret_cast<const uint8_t*>(kv.vs + at));
-        ld_words<F::NG>(f.vb[kt], reinterpret_cast<const uint8_t*>(kv.vb + at));
-      }
-    }
+    paged_load_sb<F::NG, WHOLE>(f.vs, kv.vs, row, n, c);
+    paged_load_sb<F::NG, WHOLE>(f.vb, kv.vb, row, n, c);
   }
 }
 // scale or bias of key 2c+e, group gr, from the packed pairs of one key tile
@@ -667,8 +690,9 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
       const int r = r0 + 8 * k, t = r / a.G;
       const bool live = t < z.nnew;
       const int pos = __ldg(a.b.kv_len + seq) - z.nnew + t;
-      khi[k] = live ? min(pos + 1, z.len) : 0;
-      klo[k] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      // rows of nobody are not stored; they count as seeing everything
+      khi[k] = live ? min(pos + 1, z.len) : 0x7fffffff;
+      klo[k] = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
 #pragma unroll
       for (int w = 0; w < QW; ++w) qf[k][w] = 0;
       if (live) {
@@ -704,6 +728,20 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
         }
       }
     }
+    if constexpr (BITS == 8) {  // fp16 queries (saturating) against fp16 codes
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int w = 0; w < QW; ++w) {
+          float x = lo_bf(qf[k][w]), y = hi_bf(qf[k][w]);
+          x = x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+          y = y > 65504.0f ? 65504.0f : y < -65504.0f ? -65504.0f : y;
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(qf[k][w]) : "f"(y), "f"(x));
+        }
+    }
+    // steps below / from here on need no mask for any row
+    const int all_hi = __reduce_min_sync(0xffffffffu, min(khi[0], khi[1]));
+    const int all_lo = __reduce_max_sync(0xffffffffu, max(klo[0], klo[1]));
     float o[NG][8][4];
 #pragma unroll
     for (int i = 0; i < NG; ++i)
@@ -723,13 +761,22 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
       return r < 0 ? -1 : r + (int64_t)h * a.kv.P;
     };
     F f;
+    auto load_k = [&](int64_t row, int cnt) {
+      if (cnt >= 16 && row >= 0) paged_load_k<D, BITS, true>(f, a.kv, row, cnt, g, c);
+      else paged_load_k<D, BITS, false>(f, a.kv, row, cnt, g, c);
+    };
+    auto load_v = [&](int64_t row, int cnt) {
+      if (cnt >= 16 && row >= 0) paged_load_v<D, BITS, true>(f, a.kv, row, cnt, g, c);
+      else paged_load_v<D, BITS, false>(f, a.kv, row, cnt, g, c);
+    };
     int cnt;
-    int64_t row = row_of(b0, cnt);
-    paged_load_k<D, BITS>(f, a.kv, row, cnt, g, c);
-    paged_load_v<D, BITS>(f, a.kv, row, cnt, g, c);
+    {
+      const int64_t row = row_of(b0, cnt);
+      load_k(row, cnt);
+      load_v(row, cnt);
+    }
     for (int b = b0; b < b1; ++b) {
-      int ncnt;
-      const int64_t nrow = row_of(b + 1, ncnt);
+      const int64_t nrow = row_of(b + 1, cnt);
       float s[2][4];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -744,60 +791,67 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
           for (int i = 0; i < NG; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // k16 steps of the group
-              uint32_t k0, k1;
-              if constexpr (BITS == 8) {
-                const uint32_t w = f.k[kt][4 * i + j];
-                k0 = code8_pair(__byte_perm(w, 0, 0x4140));
-                k1 = code8_pair(__byte_perm(w, 0, 0x4342));
-              } else {  // exact 128 + code
-                const uint32_t w = f.k[kt][2 * i + (j >> 1)] >> (8 * (j & 1));
-                k0 = (w & 0x000F000Fu) | 0x43004300u;
-                k1 = ((w >> 4) & 0x000F000Fu) | 0x43004300u;
-              }
               const int w = 8 * i + 2 * j;
-              mma_bf16(sg[i], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], k0, k1);
+              if constexpr (BITS == 8) {  // exact fp16 1024 + code
+                const uint32_t x = f.k[kt][4 * i + j];
+                mma_f16(sg[i], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], __byte_perm(x, 0x64646464u, 0x4140),
+                        __byte_perm(x, 0x64646464u, 0x4342));
+              } else {  // exact bf16 128 + code
+                const uint32_t x = f.k[kt][2 * i + (j >> 1)] >> (8 * (j & 1));
+                mma_bf16(sg[i], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], (x & 0x000F000Fu) | 0x43004300u,
+                         ((x >> 4) & 0x000F000Fu) | 0x43004300u);
+              }
             }
           }
-          constexpr float Z = BITS == 8 ? 128.0f : -128.0f;
+          constexpr float Z = BITS == 8 ? -1024.0f : -128.0f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[kt][e] = 0.0f;
+          for (int e = 0; e < 2; ++e) {
+            float sc[NG], bi[NG];
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-              const float sc = pair_at<NG>(f.ks[kt], e & 1, i), bi = __fmaf_rn(Z, sc, pair_at<NG>(f.kb[kt], e & 1, i));
-              s[kt][e] = __fmaf_rn(sc, sg[i][e], __fmaf_rn(bi, qs[e >> 1][i], s[kt][e]));
+              sc[i] = pair_at<NG>(f.ks[kt], e, i);
+              bi[i] = __fmaf_rn(Z, sc[i], pair_at<NG>(f.kb[kt], e, i));
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float x = bi[0] * qs[k][0];
+#pragma unroll
+              for (int i = 1; i < NG; ++i) x = __fmaf_rn(bi[i], qs[k][i], x);
+#pragma unroll
+              for (int i = 0; i < NG; ++i) x = __fmaf_rn(sc[i], sg[i][2 * k + e], x);
+              s[kt][2 * k + e] = x;
             }
           }
         }
       }
-      paged_load_k<D, BITS>(f, a.kv, nrow, ncnt, g, c);
+      load_k(nrow, cnt);
 
-      // scores in base 2; keys a row does not see at -infinity
-      const int key = z.lo + b * kPagedKeys + warp * 16 + 2 * c;
-      float mx[2] = {-INFINITY, -INFINITY};
+      // keys a row does not see at -infinity
+      const int key = z.lo + b * kPagedKeys + warp * 16;
+      if (key + 16 > all_hi || key < all_lo) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = key + 8 * kt + (e & 1), k = e >> 1;
-          s[kt][e] = j < khi[k] && j >= klo[k] ? __fmul_rn(s[kt][e], a.scale2) : -INFINITY;
-          mx[k] = fmaxf(mx[k], s[kt][e]);
-        }
+          for (int e = 0; e < 4; ++e) {
+            const int j = key + 2 * c + 8 * kt + (e & 1), k = e >> 1;
+            if (j >= khi[k] || j < klo[k]) s[kt][e] = -INFINITY;
+          }
+      }
       float msafe[2];
       bool grow = false;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
-        mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
-        mx[k] = fmaxf(mx[k], m[k]);
-        grow = grow || mx[k] != m[k];
-        msafe[k] = mx[k] == -INFINITY ? 0.0f : mx[k];
+        float mx = fmaxf(fmaxf(s[0][2 * k], s[0][2 * k + 1]), fmaxf(s[1][2 * k], s[1][2 * k + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * a.scale2;
+        grow = grow || mx > m[k];
+        msafe[k] = fmaxf(mx, m[k]);
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float al = ex2f(m[k] - msafe[k]);
-          m[k] = mx[k];
+          const float al = m[k] == msafe[k] ? 1.0f : ex2f(m[k] - msafe[k]);
+          m[k] = msafe[k];
           l[k] *= al;
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
@@ -812,10 +866,12 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
       }
       float p[2][4];
 #pragma unroll
+      for (int k = 0; k < 2; ++k) msafe[k] = m[k] == -INFINITY ? 0.0f : -m[k];
+#pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[kt][e] = ex2f(s[kt][e] - msafe[e >> 1]);
+          p[kt][e] = ex2f(__fmaf_rn(s[kt][e], a.scale2, msafe[e >> 1]));
           l[e >> 1] += p[kt][e];
         }
 #pragma unroll
@@ -823,27 +879,28 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
         // A fragments: a0 (row g, keys 0..7) a1 (row g+8) a2 (row g, keys 8..15) a3
         uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt) {
+          float sv[2] = {1.0f, 1.0f}, bv[2] = {0.0f, 0.0f};
+          if constexpr (BITS != 16) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              sv[e] = pair_at<NG>(f.vs[kt], e, i);
+              bv[e] = __fmaf_rn(BITS == 8 ? 128.0f : 8.0f, sv[e], pair_at<NG>(f.vb[kt], e, i));
+            }
+          }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             float x0 = p[kt][2 * k], x1 = p[kt][2 * k + 1];
             if constexpr (BITS != 16) {
-              constexpr float Z = BITS == 8 ? 128.0f : 8.0f;
-              const float s0 = pair_at<NG>(f.vs[kt], 0, i), s1 = pair_at<NG>(f.vs[kt], 1, i);
-              // a key that the row does not see has p = 0 and may hold any scale
-              if (x0 != 0.0f) {
-                vbs[k][i] = __fmaf_rn(x0, __fmaf_rn(Z, s0, pair_at<NG>(f.vb[kt], 0, i)), vbs[k][i]);
-                x0 *= s0;
-              }
-              if (x1 != 0.0f) {
-                vbs[k][i] = __fmaf_rn(x1, __fmaf_rn(Z, s1, pair_at<NG>(f.vb[kt], 1, i)), vbs[k][i]);
-                x1 *= s1;
-              }
+              vbs[k][i] = __fmaf_rn(x1, bv[1], __fmaf_rn(x0, bv[0], vbs[k][i]));
+              x0 *= sv[0];
+              x1 *= sv[1];
             }
             const uint32_t hi = pk_bf2(x0, x1);
             ph[2 * kt + k] = hi;
             pl[2 * kt + k] = pk_bf2(x0 - lo_bf(hi), x1 - hi_bf(hi));
           }
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint32_t vv[2];
@@ -863,9 +920,7 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
           mma_bf16(o[i][j], pl[0], pl[1], pl[2], pl[3], vv[0], vv[1]);
         }
       }
-      paged_load_v<D, BITS>(f, a.kv, nrow, ncnt, g, c);
-      row = nrow;
-      cnt = ncnt;
+      load_v(nrow, cnt);
     }
 
     // the four warps' results meet: sums over the lanes of a row, then
@@ -949,17 +1004,18 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
   }
 }
 
-// Join of the items that several CTAs share: a warp per (token, head).  The
-// contributors of blocks [i0, i1) are CTAs c0 .. c1; only c0 can have begun
-// in an earlier item (its slot 1), the others begin inside this one.
+// Join of the items that several CTAs share: a CTA per (token, head), its four
+// warps taking every fourth contributor.  The contributors of blocks [i0, i1)
+// are CTAs c0 .. c1; only c0 can have begun in an earlier item (its slot 1),
+// the others begin inside this one.
 template <int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(PagedAttnArgs a) {
+  constexpr int V = D / 32;
+  __shared__ float s_m[4], s_l[4], s_o[4][D];
   grid_wait();
   grid_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (int64_t)a.b.tokens * a.heads) return;
-  const int t = (int)(w / a.heads), head = (int)(w % a.heads);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t = (int)(blockIdx.x / a.heads), head = (int)(blockIdx.x % a.heads);
   const int seq = paged_seq(a.b, t, lane);
   if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;
   const PagedSpan z = paged_span(a, seq);
@@ -967,34 +1023,51 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(PagedAttnArgs a) {
   const int64_t total = a.prefix[a.b.seqs], n = total < a.nctas ? total : a.nctas;
   const int64_t i0 = a.prefix[seq] + ((int64_t)h * z.tiles + r / 16) * z.nblk, i1 = i0 + z.nblk;
   // CTA c owns blocks [total*c/n, total*(c+1)/n)
-  const int64_t c0 = ((i0 + 1) * n - 1) / total, c1 = (i1 * n - 1) / total;
+  const int c0 = (int)(((i0 + 1) * n - 1) / total), c1 = (int)((i1 * n - 1) / total);
   if (c0 == c1) return;  // written by its CTA
-  auto slot_of = [&](int64_t cta) { return 2 * cta + (cta == c0 && total * cta / n < i0 ? 1 : 0); };
-  float M = -INFINITY;
-  for (int64_t k = c0 + lane; k <= c1; k += 32) M = fmaxf(M, a.ml[(slot_of(k) * 16 + r % 16) * 2]);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  const float ms = M == -INFINITY ? 0.0f : M;
-  constexpr int V = D / 32;
-  float L = 0.0f, acc[V] = {};
+  const int slot0 = 2 * c0 + (total * c0 / n < i0 ? 1 : 0);
+  float M = -INFINITY, L = 0.0f, acc[V] = {};
 #pragma unroll 4
-  for (int64_t k = c0; k <= c1; ++k) {
-    const int64_t s = slot_of(k) * 16 + r % 16;
+  for (int k = c0 + warp; k <= c1; k += 4) {
+    const int64_t s = (int64_t)(k == c0 ? slot0 : 2 * k) * 16 + r % 16;
     const float2 ml = *reinterpret_cast<const float2*>(a.ml + s * 2);
-    const float wt = ex2f(ml.x - ms);
-    L = __fmaf_rn(wt, ml.y, L);
+    float x[V];
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(a.part + s * D + lane * V + e);
-      acc[e] = __fmaf_rn(wt, x.x, acc[e]);
-      acc[e + 1] = __fmaf_rn(wt, x.y, acc[e + 1]);
+      const float2 y = *reinterpret_cast<const float2*>(a.part + s * D + lane * V + e);
+      x[e] = y.x;
+      x[e + 1] = y.y;
     }
+    const float mn = fmaxf(M, ml.x), ms = mn == -INFINITY ? 0.0f : mn;
+    const float w0 = ex2f(M - ms), w1 = ex2f(ml.x - ms);
+    M = mn;
+    L = __fmaf_rn(w1, ml.y, L * w0);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = __fmaf_rn(w1, x[e], acc[e] * w0);
+  }
+  if (lane == 0) {
+    s_m[warp] = M;
+    s_l[warp] = L;
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) s_o[warp][lane * V + e] = acc[e];
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float ms = M == -INFINITY ? 0.0f : M;
+  float y0 = 0.0f, y1 = 0.0f;
+  L = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float wt = ex2f(s_m[k] - ms);
+    L = __fmaf_rn(wt, s_l[k], L);
+    y0 = __fmaf_rn(wt, s_o[k][2 * threadIdx.x], y0);
+    y1 = __fmaf_rn(wt, s_o[k][2 * threadIdx.x + 1], y1);
   }
   const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
-  bf16_t* op = a.out + (int64_t)t * a.ldo + (int64_t)head * D + lane * V;
-#pragma unroll
-  for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(op + e) = pk_bf2(acc[e] * inv, acc[e + 1] * inv);
-  if (a.lse && lane == 0)
+  bf16_t* op = a.out + (int64_t)t * a.ldo + (int64_t)head * D + 2 * threadIdx.x;
+  *reinterpret_cast<uint32_t*>(op) = pk_bf2(y0 * inv, y1 * inv);
+  if (a.lse && threadIdx.x == 0)
     a.lse[(int64_t)t * a.heads + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
 }
 

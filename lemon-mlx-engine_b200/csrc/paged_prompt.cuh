@@ -467,17 +467,18 @@ LMX_DEV uint4 prompt_q8(uint4 v) {
 }
 // the output columns back in order
 template <int BITS>
-LMX_DEV void prompt_order(float* y) {
-  if (BITS != 4) return;
+LMX_DEV void prompt_order(float (&y)[16]) {
+  if constexpr (BITS == 4) {
 #pragma unroll
-  for (int k = 0; k < 16; k += 8) {
-    float t[8];
+    for (int k = 0; k < 16; k += 8) {
+      float t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = y[k + i];
+      for (int i = 0; i < 8; ++i) t[i] = y[k + i];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[k + i] = t[2 * i];
-      y[k + i + 4] = t[2 * i + 1];
+      for (int i = 0; i < 4; ++i) {
+        y[k + i] = t[2 * i];
+        y[k + i + 4] = t[2 * i + 1];
+      }
     }
   }
 }

@@ -2,6 +2,7 @@
 // operators (include/lmx.h, "Paged KV cache").
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "lmx_internal.h"
 #include <cudaTypedefs.h>
@@ -244,28 +245,43 @@ int g_prompt_min_rows = 33;
 
 struct AttnPlan {
   bool prompt = false;
+  int rows = 0;  // query rows of an item
   int nctas = 0;
   size_t start = 0, ml = 0, part = 0, bytes = 0;  // offsets into the scratch
 };
 
-template <int D, int BITS>
+template <int D, int BITS, int NT>
 int few_rows_ctas(int* n) {
   static int per[64] = {};
   int d = 0;
   cudaGetDevice(&d);
   if (!per[d & 63]) {
     const int most = (kPagedMaxSeqs + 1) * 8;
-    int rc = cuda_check(cudaFuncSetAttribute(paged_attn_kernel<D, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
+    int rc = cuda_check(cudaFuncSetAttribute(paged_attn_kernel<D, BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
                         "paged_attention: set smem");
     int c = 0;
     if (!rc)
-      rc = cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c, paged_attn_kernel<D, BITS>, 128, most),
+      rc = cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c, paged_attn_kernel<D, BITS, NT>, 128, most),
                       "paged_attention: occupancy");
     if (rc) return rc;
     per[d & 63] = c > 0 ? c : 1;
   }
   *n = per[d & 63] * device_sms();
   return LMX_OK;
+}
+
+// f(head dim, bits, 8-row tiles) as compile-time constants
+template <typename F>
+int few_rows(int D, int bits, int rows, F f) {
+  auto nt = [&](auto d, auto b) {
+    return rows == 8 ? f(d, b, std::integral_constant<int, 1>()) : f(d, b, std::integral_constant<int, 2>());
+  };
+  auto on_bits = [&](auto d) {
+    return bits == 16  ? nt(d, std::integral_constant<int, 16>())
+           : bits == 8 ? nt(d, std::integral_constant<int, 8>())
+                       : nt(d, std::integral_constant<int, 4>());
+  };
+  return D == 64 ? on_bits(std::integral_constant<int, 64>()) : on_bits(std::integral_constant<int, 128>());
 }
 
 int check_attn(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads, AttnPlan& p) {
@@ -278,21 +294,21 @@ int check_attn(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads, 
   const int D = kv->head_dim;
   p.prompt = g_prompt_min_rows > 0 &&
              (int64_t)batch->max_new * (heads / kv->kv_heads) >= g_prompt_min_rows;
-  int rows = 16;  // of a partial result
   if (p.prompt) {
-    rows = kPromptRows;
+    p.rows = kPromptRows;
     p.nctas = device_sms();
-  } else if (D == 64) {
-    rc = kv->bits == 16 ? few_rows_ctas<64, 16>(&p.nctas) : kv->bits == 8 ? few_rows_ctas<64, 8>(&p.nctas) : few_rows_ctas<64, 4>(&p.nctas);
   } else {
-    rc = kv->bits == 16 ? few_rows_ctas<128, 16>(&p.nctas) : kv->bits == 8 ? few_rows_ctas<128, 8>(&p.nctas) : few_rows_ctas<128, 4>(&p.nctas);
+    p.rows = (int64_t)batch->max_new * (heads / kv->kv_heads) <= 8 ? 8 : 16;
+    rc = few_rows(D, kv->bits, p.rows, [&](auto d, auto bits, auto nt) {
+      return few_rows_ctas<decltype(d)::value, decltype(bits)::value, decltype(nt)::value>(&p.nctas);
+    });
   }
   if (rc) return rc;
   auto after = [](size_t at, size_t bytes) { return (at + bytes + 255) / 256 * 256; };
   p.start = after(0, (size_t)(batch->seqs + 1) * 8);
   p.ml = after(p.start, p.prompt ? (size_t)p.nctas * sizeof(int4) : 0);
-  p.part = after(p.ml, (size_t)2 * p.nctas * rows * 2 * 4);
-  p.bytes = p.part + (size_t)2 * p.nctas * rows * D * 4;
+  p.part = after(p.ml, (size_t)2 * p.nctas * p.rows * 2 * 4);
+  p.bytes = p.part + (size_t)2 * p.nctas * p.rows * D * 4;
   return LMX_OK;
 }
 
@@ -360,9 +376,9 @@ int launch_prompt(const PagedAttnArgs& a, const AttnPlan& pl, cudaStream_t st) {
   return rc;
 }
 
-template <int D, int BITS>
+template <int D, int BITS, int NT>
 int launch_few(const PagedAttnArgs& a, cudaStream_t st) {
-  int rc = cuda_check(lmx_launch(paged_attn_kernel<D, BITS>, dim3(a.nctas), dim3(128), (size_t)(a.b.seqs + 1) * 8, st, true, a),
+  int rc = cuda_check(lmx_launch(paged_attn_kernel<D, BITS, NT>, dim3(a.nctas), dim3(128), (size_t)(a.b.seqs + 1) * 8, st, true, a),
                       "paged_attention: launch");
   if (rc) return rc;
   unsigned grid;
@@ -417,6 +433,7 @@ extern "C" int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch
   a.prefix = (int64_t*)scratch;
   a.ml = (float*)((uint8_t*)scratch + p.ml);
   a.part = (float*)((uint8_t*)scratch + p.part);
+  a.rows = p.rows;
   a.nctas = p.nctas;
   a.err = device_error_word();
   cudaStream_t st = (cudaStream_t)stream;
@@ -425,7 +442,7 @@ extern "C" int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch
       return kv->bits == 16 ? launch_prompt<64, 16>(a, p, st) : kv->bits == 8 ? launch_prompt<64, 8>(a, p, st) : launch_prompt<64, 4>(a, p, st);
     return kv->bits == 16 ? launch_prompt<128, 16>(a, p, st) : kv->bits == 8 ? launch_prompt<128, 8>(a, p, st) : launch_prompt<128, 4>(a, p, st);
   }
-  if (D == 64)
-    return kv->bits == 16 ? launch_few<64, 16>(a, st) : kv->bits == 8 ? launch_few<64, 8>(a, st) : launch_few<64, 4>(a, st);
-  return kv->bits == 16 ? launch_few<128, 16>(a, st) : kv->bits == 8 ? launch_few<128, 8>(a, st) : launch_few<128, 4>(a, st);
+  return few_rows(D, kv->bits, p.rows, [&](auto d, auto bits, auto nt) {
+    return launch_few<decltype(d)::value, decltype(bits)::value, decltype(nt)::value>(a, st);
+  });
 }

@@ -431,8 +431,12 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
 // Attention, few query rows per KV head.
 //
 // The G query heads of a KV head times its sequence's new tokens are rows
-// r = t*G + g, tiled by 16: one m16 MMA row tile, so a tile's rows share one
-// pass over the sequence's rows of that head.  Bound by the cache bytes.
+// r = t*G + g, tiled by 8 or 16, so a tile's rows share one pass over the
+// sequence's rows of that head.  Bound by the cache bytes.  The products run
+// transposed, S^T = K Q^T and O^T = V^T P^T: the 16-row side of mma.m16n8k16
+// is then keys and head dims, which are plenty, and the query rows are its
+// 8-wide side, so eight rows (a decode step of G <= 8) waste nothing and their
+// accumulators and queries take half the registers of 16.
 //
 // Work split: an item is (sequence, head, tile); its key range is cut into
 // blocks of 64 keys, and the blocks of all items, laid end to end, are divided
@@ -445,10 +449,11 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
 // Within a block each of the four warps takes 16 keys and runs its own
 // online softmax; the warps meet once per item, in shared memory.  K and V
 // go from global memory straight to MMA fragments: the contraction order of
-// q.k is free, so a lane's B fragments are 8 (16 when quantized) consecutive
-// values of a key, Q being laid out the same way; and the output column
-// order is free, so a lane's V fragments are 8 consecutive values of four
-// keys, paired by byte permutes.  The next block's K loads are issued when the
+// q.k is free, so a lane's K fragments are 8 (16 when quantized) consecutive
+// values of two keys, Q being laid out the same way; and the order of the
+// head dims is free, so a lane's V fragments are 8 consecutive values of four
+// keys, paired by byte permutes; P^T is S^T with its 8 x 8 blocks transposed
+// (movmatrix).  The next block's K loads are issued when the
 // scores are done, its V loads when P V is done, so loads stay in flight
 // through the arithmetic without a second set of registers.
 //
@@ -477,8 +482,9 @@ struct PagedAttnArgs {
   int64_t ldo;
   float* lse;
   int64_t* prefix;  // scratch: blocks before each sequence [seqs + 1]
-  float* ml;        // [2 * grid][16][2]
-  float* part;      // [2 * grid][16][D]
+  float* ml;        // [2 * grid][rows][2]
+  float* part;      // [2 * grid][rows][D]
+  int rows;         // query rows of a tile (few-row kernel: 8 or 16)
   int nctas;
   unsigned* err;
 };
@@ -497,7 +503,7 @@ LMX_DEV PagedSpan paged_span(const PagedAttnArgs& a, int s) {
   z.len = (int)min((int64_t)max(__ldg(a.b.kv_len + s), 0), cap);
   z.lo = 0;
   if (a.window > 0) z.lo = max(0, __ldg(a.b.kv_len + s) - z.nnew - a.window + 1) & ~15;
-  z.tiles = (int)(((int64_t)z.nnew * a.G + 15) / 16);
+  z.tiles = (int)(((int64_t)z.nnew * a.G + a.rows - 1) / a.rows);
   z.nblk = max(1, (max(z.len - z.lo, 0) + kPagedKeys - 1) / kPagedKeys);
   return z;
 }
@@ -531,12 +537,11 @@ LMX_DEV void paged_prefix(const PagedAttnArgs& a, int64_t* pre, int64_t* wsum) {
 
 template <int D, int BITS>
 struct PagedFrag {
-  static constexpr int NG = D / 64;
   static constexpr int KW = BITS == 16 ? D / 8 : (BITS == 8 ? D / 16 : D / 32);  // words of one key's lane share
   static constexpr int VW = BITS == 16 ? D / 16 : (BITS == 8 ? D / 32 : D / 64);  // words of one V row's lane share
-  uint32_t k[2][KW];
-  uint32_t v[4][VW];
-  uint32_t ks[2][NG], kb[2][NG], vs[2][NG], vb[2][NG];  // bf16 pairs (quantized)
+  uint32_t k[2][KW];                  // keys g, g + 8
+  uint32_t v[4][VW];                  // keys 2c, 2c + 1, 2c + 8, 2c + 9
+  uint32_t ks[2], kb[2], vs[2], vb[2];  // keys g, g + 8: bf16 of the one or two groups (quantized)
 };
 
 template <int N>
@@ -552,23 +557,15 @@ LMX_DEV void ld_words(uint32_t* d, const uint8_t* p) {
   }
 }
 
-// scales or biases of keys 2c, 2c+1 (+ 8 kt) from `base`, row `row`; keys past n
-// get zeros, whatever the page holds there
+// scales or biases of keys g, g + 8; keys past n get zeros, whatever the page
+// holds there
 template <int NG, bool WHOLE>
-LMX_DEV void paged_load_sb(uint32_t (&d)[2][NG], const bf16_t* base, int64_t row, int n, int c) {
+LMX_DEV void paged_load_sb(uint32_t (&d)[2], const bf16_t* base, int64_t row, int n, int g) {
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    const int key = 8 * kt + 2 * c;
-    ld_words<NG>(d[kt], reinterpret_cast<const uint8_t*>(base + (row + key) * NG));
-    if constexpr (!WHOLE) {
-      if constexpr (NG == 2) {
-        if (key >= n) d[kt][0] = 0;
-        if (key + 1 >= n) d[kt][1] = 0;
-      } else {
-        if (key >= n) d[kt][0] = 0;
-        if (key + 1 >= n) d[kt][0] &= 0xffffu;
-      }
-    }
+    const bf16_t* p = base + (row + 8 * kt + g) * NG;
+    d[kt] = 0;
+    if (WHOLE || 8 * kt + g < n) d[kt] = NG == 2 ? __ldg(reinterpret_cast<const uint32_t*>(p)) : (uint32_t)__ldg(p);
   }
 }
 // K fragments (and the quantizer's scales and biases) of the 16 keys whose
@@ -594,8 +591,8 @@ LMX_DEV void paged_load_k(PagedFrag<D, BITS>& f, const PagedKv& kv, int64_t row,
       for (int i = 0; i < RB / CH; ++i) ld_words<CH / 16>(f.k[kt] + i * (CH / 16), p + 8 * kt * RB + i * CH);
   }
   if constexpr (BITS != 16) {
-    paged_load_sb<F::NG, WHOLE>(f.ks, kv.ks, row, n, c);
-    paged_load_sb<F::NG, WHOLE>(f.kb, kv.kb, row, n, c);
+    paged_load_sb<D / 64, WHOLE>(f.ks, kv.ks, row, n, g);
+    paged_load_sb<D / 64, WHOLE>(f.kb, kv.kb, row, n, g);
   }
 }
 // V fragments: rows 2c, 2c+1, 2c+8, 2c+9
@@ -619,15 +616,9 @@ LMX_DEV void paged_load_v(PagedFrag<D, BITS>& f, const PagedKv& kv, int64_t row,
       for (int i = 0; i < D / 64; ++i) ld_words<CH / 32>(f.v[r] + i * (CH / 32), p + key * RB + i * CH);
   }
   if constexpr (BITS != 16) {
-    paged_load_sb<F::NG, WHOLE>(f.vs, kv.vs, row, n, c);
-    paged_load_sb<F::NG, WHOLE>(f.vb, kv.vb, row, n, c);
+    paged_load_sb<D / 64, WHOLE>(f.vs, kv.vs, row, n, g);
+    paged_load_sb<D / 64, WHOLE>(f.vb, kv.vb, row, n, g);
   }
-}
-// scale or bias of key 2c+e, group gr, from the packed pairs of one key tile
-template <int NG>
-LMX_DEV float pair_at(const uint32_t (&w)[NG], int e, int gr) {
-  if constexpr (NG == 2) return gr ? hi_bf(w[e]) : lo_bf(w[e]);
-  else return e ? hi_bf(w[0]) : lo_bf(w[0]);
 }
 // two bytes in the low bytes of the 16-bit halves of t -> exact bf16 pair
 // (code - 128): 0x4300 | low seven bits is 128 + them, and the number to
@@ -637,15 +628,27 @@ LMX_DEV uint32_t code8_pair(uint32_t t) {
   return bf2_fma3(z, 0xBF80BF80u, x);
 }
 
-template <int D, int BITS>
-__global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedAttnArgs a) {
+// 8 x 8 16-bit matrix, lane (g, c) holding row g, columns 2c and 2c + 1 -> its transpose
+LMX_DEV uint32_t movm_t(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+LMX_DEV float half_bf(uint32_t w, int i) { return i ? hi_bf(w) : lo_bf(w); }
+
+#ifndef FEWCTA
+#define FEWCTA 3
+#endif
+// NT: 8-row tiles of query rows
+template <int D, int BITS, int NT>
+__global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) paged_attn_kernel(PagedAttnArgs a) {
   using F = PagedFrag<D, BITS>;
   constexpr int NG = D / 64, QW = D / 8;  // Q words per lane and row
-  constexpr int OP = D + 4;               // pitch of the merge buffer
+  constexpr int R = 8 * NT, OP = D + 4;   // rows, pitch of the merge buffer
   extern __shared__ int64_t pre[];
   __shared__ int64_t wsum[4];
-  __shared__ float sm_m[4][16], sm_l[4][16];
-  __shared__ __align__(16) float sm_o[4][16][OP];
+  __shared__ float sm_m[4][R], sm_l[4][R];
+  __shared__ __align__(16) float sm_o[4][R][OP];
   grid_wait();
   grid_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -680,31 +683,25 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
     const int b0 = (int)(loc % z.nblk), tile = (int)(loc / z.nblk % z.tiles), h = (int)(loc / z.nblk / z.tiles);
     const int b1 = (int)min((int64_t)z.nblk, b0 + (end - at));
 
-    // rows of this lane: g and g + 8 of the tile
-    const int r0 = tile * 16 + g;
-    int klo[2], khi[2];
-    uint32_t qf[2][QW];
-    float qs[2][NG];
+    // a lane's query fragments are of rows 8 nt + g, its scores of rows 8 nt + 2c, + 1
+    const int kvlen = __ldg(a.b.kv_len + seq);
+    uint32_t qf[NT][QW];
+    float qs[NT][2][NG];  // sums of a row's queries per group
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int r = r0 + 8 * k, t = r / a.G;
-      const bool live = t < z.nnew;
-      const int pos = __ldg(a.b.kv_len + seq) - z.nnew + t;
-      // rows of nobody are not stored; they count as seeing everything
-      khi[k] = live ? min(pos + 1, z.len) : 0x7fffffff;
-      klo[k] = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = tile * R + 8 * nt + g, t = r / a.G;
 #pragma unroll
-      for (int w = 0; w < QW; ++w) qf[k][w] = 0;
-      if (live) {
+      for (int w = 0; w < QW; ++w) qf[nt][w] = 0;
+      if (t < z.nnew) {
         const bf16_t* qp = a.q + (int64_t)(z.first + t) * a.ldq + (int64_t)(h * a.G + r % a.G) * D;
         if constexpr (BITS == 16) {
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) ld_words<4>(qf[k] + 4 * i, reinterpret_cast<const uint8_t*>(qp + 32 * i + 8 * c));
+          for (int i = 0; i < D / 32; ++i) ld_words<4>(qf[nt] + 4 * i, reinterpret_cast<const uint8_t*>(qp + 32 * i + 8 * c));
         } else {
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
-            ld_words<4>(qf[k] + 8 * i, reinterpret_cast<const uint8_t*>(qp + 64 * i + 16 * c));
-            ld_words<4>(qf[k] + 8 * i + 4, reinterpret_cast<const uint8_t*>(qp + 64 * i + 16 * c + 8));
+            ld_words<4>(qf[nt] + 8 * i, reinterpret_cast<const uint8_t*>(qp + 64 * i + 16 * c));
+            ld_words<4>(qf[nt] + 8 * i + 4, reinterpret_cast<const uint8_t*>(qp + 64 * i + 16 * c + 8));
           }
         }
       }
@@ -713,43 +710,66 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
         for (int i = 0; i < NG; ++i) {
           float sum = 0.0f;
 #pragma unroll
-          for (int w = 0; w < 8; ++w) sum += lo_bf(qf[k][8 * i + w]) + hi_bf(qf[k][8 * i + w]);
-          qs[k][i] = warp_sum_xor(sum, 2, 1);
+          for (int w = 0; w < 8; ++w) sum += lo_bf(qf[nt][8 * i + w]) + hi_bf(qf[nt][8 * i + w]);
+          sum = warp_sum_xor(sum, 2, 1);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) qs[nt][e][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * c + e));
         }
       }
       if constexpr (BITS == 4) {  // a word's nibbles come out as pairs (0,4) (1,5) (2,6) (3,7)
 #pragma unroll
         for (int w = 0; w < QW; w += 4) {
-          const uint32_t w0 = qf[k][w], w1 = qf[k][w + 1], w2 = qf[k][w + 2], w3 = qf[k][w + 3];
-          qf[k][w] = __byte_perm(w0, w2, 0x5410);
-          qf[k][w + 1] = __byte_perm(w0, w2, 0x7632);
-          qf[k][w + 2] = __byte_perm(w1, w3, 0x5410);
-          qf[k][w + 3] = __byte_perm(w1, w3, 0x7632);
+          const uint32_t w0 = qf[nt][w], w1 = qf[nt][w + 1], w2 = qf[nt][w + 2], w3 = qf[nt][w + 3];
+          qf[nt][w] = __byte_perm(w0, w2, 0x5410);
+          qf[nt][w + 1] = __byte_perm(w0, w2, 0x7632);
+          qf[nt][w + 2] = __byte_perm(w1, w3, 0x5410);
+          qf[nt][w + 3] = __byte_perm(w1, w3, 0x7632);
+        }
+      }
+      if constexpr (BITS == 8) {  // fp16 queries (saturating) against fp16 codes
+#pragma unroll
+        for (int w = 0; w < QW; ++w) {
+          float x = lo_bf(qf[nt][w]), y = hi_bf(qf[nt][w]);
+          x = x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+          y = y > 65504.0f ? 65504.0f : y < -65504.0f ? -65504.0f : y;
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(qf[nt][w]) : "f"(y), "f"(x));
         }
       }
     }
-    if constexpr (BITS == 8) {  // fp16 queries (saturating) against fp16 codes
+    // keys that rows 8 nt + 2c + e see; rows of nobody are not stored and count
+    // as seeing everything
+    int khi[NT][2], klo[NT][2], all_hi = 0x7fffffff, all_lo = 0;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int w = 0; w < QW; ++w) {
-          float x = lo_bf(qf[k][w]), y = hi_bf(qf[k][w]);
-          x = x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
-          y = y > 65504.0f ? 65504.0f : y < -65504.0f ? -65504.0f : y;
-          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(qf[k][w]) : "f"(y), "f"(x));
-        }
-    }
+      for (int e = 0; e < 2; ++e) {
+        const int t = (tile * R + 8 * nt + 2 * c + e) / a.G, pos = kvlen - z.nnew + t;
+        const bool live = t < z.nnew;
+        khi[nt][e] = live ? min(pos + 1, z.len) : 0x7fffffff;
+        klo[nt][e] = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        all_hi = min(all_hi, khi[nt][e]);
+        all_lo = max(all_lo, klo[nt][e]);
+      }
     // steps below / from here on need no mask for any row
-    const int all_hi = __reduce_min_sync(0xffffffffu, min(khi[0], khi[1]));
-    const int all_lo = __reduce_max_sync(0xffffffffu, max(klo[0], klo[1]));
-    float o[NG][8][4];
+    all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+    all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+    float o[NT][NG][4][4];  // head dims 64 i + 8 g + j (+ 4), rows 2c, 2c + 1
 #pragma unroll
-    for (int i = 0; i < NG; ++i)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int i = 0; i < NG; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][j][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, vbs[2][NG] = {};
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][i][j][e] = 0.0f;
+    float m[NT][2], l[NT][2], vbs[NT][2][NG] = {};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[nt][e] = -INFINITY;
+        l[nt][e] = 0.0f;
+      }
 
     // step b: keys [lo + 64 b + 16 warp, +16); its row of head h, or -1
     auto row_of = [&](int b, int& cnt) -> int64_t {
@@ -777,51 +797,62 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
     }
     for (int b = b0; b < b1; ++b) {
       const int64_t nrow = row_of(b + 1, cnt);
-      float s[2][4];
+      // s[nt]: key g rows 2c, 2c + 1, then key g + 8
+      float s[NT][4];
+      if constexpr (BITS == 16) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        if constexpr (BITS == 16) {
-          s[kt][0] = s[kt][1] = s[kt][2] = s[kt][3] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt) {
+          s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
           for (int w = 0; w < QW; w += 2)
-            mma_bf16(s[kt], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], f.k[kt][w], f.k[kt][w + 1]);
-        } else {
-          float sg[NG][4] = {};
+            mma_bf16(s[nt], f.k[0][w], f.k[1][w], f.k[0][w + 1], f.k[1][w + 1], qf[nt][w], qf[nt][w + 1]);
+        }
+      } else {
+        float sg[NT][NG][4] = {};
 #pragma unroll
-          for (int i = 0; i < NG; ++i) {
+        for (int i = 0; i < NG; ++i) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // k16 steps of the group
-              const int w = 8 * i + 2 * j;
+          for (int j = 0; j < 4; ++j) {  // k16 steps of the group
+            uint32_t k0[2], k1[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
               if constexpr (BITS == 8) {  // exact fp16 1024 + code
                 const uint32_t x = f.k[kt][4 * i + j];
-                mma_f16(sg[i], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], __byte_perm(x, 0x64646464u, 0x4140),
-                        __byte_perm(x, 0x64646464u, 0x4342));
+                k0[kt] = __byte_perm(x, 0x64646464u, 0x4140);
+                k1[kt] = __byte_perm(x, 0x64646464u, 0x4342);
               } else {  // exact bf16 128 + code
                 const uint32_t x = f.k[kt][2 * i + (j >> 1)] >> (8 * (j & 1));
-                mma_bf16(sg[i], qf[0][w], qf[1][w], qf[0][w + 1], qf[1][w + 1], (x & 0x000F000Fu) | 0x43004300u,
-                         ((x >> 4) & 0x000F000Fu) | 0x43004300u);
+                k0[kt] = (x & 0x000F000Fu) | 0x43004300u;
+                k1[kt] = ((x >> 4) & 0x000F000Fu) | 0x43004300u;
               }
             }
-          }
-          constexpr float Z = BITS == 8 ? -1024.0f : -128.0f;
+            const int w = 8 * i + 2 * j;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float sc[NG], bi[NG];
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-              sc[i] = pair_at<NG>(f.ks[kt], e, i);
-              bi[i] = __fmaf_rn(Z, sc[i], pair_at<NG>(f.kb[kt], e, i));
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float x = bi[0] * qs[k][0];
-#pragma unroll
-              for (int i = 1; i < NG; ++i) x = __fmaf_rn(bi[i], qs[k][i], x);
-#pragma unroll
-              for (int i = 0; i < NG; ++i) x = __fmaf_rn(sc[i], sg[i][2 * k + e], x);
-              s[kt][2 * k + e] = x;
+            for (int nt = 0; nt < NT; ++nt) {
+              if constexpr (BITS == 8) mma_f16(sg[nt][i], k0[0], k0[1], k1[0], k1[1], qf[nt][w], qf[nt][w + 1]);
+              else mma_bf16(sg[nt][i], k0[0], k0[1], k1[0], k1[1], qf[nt][w], qf[nt][w + 1]);
             }
           }
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          float sc[NG], bi[NG];
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            sc[i] = half_bf(f.ks[kt], i);
+            bi[i] = __fmaf_rn(BITS == 8 ? -1024.0f : -128.0f, sc[i], half_bf(f.kb[kt], i));
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = bi[0] * qs[nt][e][0];
+#pragma unroll
+              for (int i = 1; i < NG; ++i) x = __fmaf_rn(bi[i], qs[nt][e][i], x);
+#pragma unroll
+              for (int i = 0; i < NG; ++i) x = __fmaf_rn(sc[i], sg[nt][i][2 * kt + e], x);
+              s[nt][2 * kt + e] = x;
+            }
         }
       }
       load_k(nrow, cnt);
@@ -830,94 +861,105 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
       const int key = z.lo + b * kPagedKeys + warp * 16;
       if (key + 16 > all_hi || key < all_lo) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int j = key + 2 * c + 8 * kt + (e & 1), k = e >> 1;
-            if (j >= khi[k] || j < klo[k]) s[kt][e] = -INFINITY;
+            const int j = key + g + 8 * (e >> 1);
+            if (j >= khi[nt][e & 1] || j < klo[nt][e & 1]) s[nt][e] = -INFINITY;
           }
       }
-      float msafe[2];
+      float mn[NT][2];
       bool grow = false;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float mx = fmaxf(fmaxf(s[0][2 * k], s[0][2 * k + 1]), fmaxf(s[1][2 * k], s[1][2 * k + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * a.scale2;
-        grow = grow || mx > m[k];
-        msafe[k] = fmaxf(mx, m[k]);
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+          mx *= a.scale2;
+          grow = grow || mx > m[nt][e];
+          mn[nt][e] = fmaxf(mx, m[nt][e]);
+        }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float al = m[k] == msafe[k] ? 1.0f : ex2f(m[k] - msafe[k]);
-          m[k] = msafe[k];
-          l[k] *= al;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            vbs[k][i] *= al;
+          for (int e = 0; e < 2; ++e) {
+            const float al = m[nt][e] == mn[nt][e] ? 1.0f : ex2f(m[nt][e] - mn[nt][e]);
+            m[nt][e] = mn[nt][e];
+            l[nt][e] *= al;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              o[i][j][2 * k] *= al;
-              o[i][j][2 * k + 1] *= al;
+            for (int i = 0; i < NG; ++i) {
+              vbs[nt][e][i] *= al;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                o[nt][i][j][e] *= al;
+                o[nt][i][j][2 + e] *= al;
+              }
             }
+          }
+      }
+      // p, and (bf16 caches) its two terms as P^T's fragments
+      float p[NT][4];
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ms = m[nt][e & 1] == -INFINITY ? 0.0f : -m[nt][e & 1];
+          p[nt][e] = ex2f(__fmaf_rn(s[nt][e], a.scale2, ms));
+          l[nt][e & 1] += p[nt][e];
+        }
+        if constexpr (BITS == 16) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            const uint32_t hi = pk_bf2(p[nt][2 * kt], p[nt][2 * kt + 1]);
+            ph[nt][kt] = movm_t(hi);
+            pl[nt][kt] = movm_t(pk_bf2(p[nt][2 * kt] - lo_bf(hi), p[nt][2 * kt + 1] - hi_bf(hi)));
           }
         }
       }
-      float p[2][4];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) msafe[k] = m[k] == -INFINITY ? 0.0f : -m[k];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[kt][e] = ex2f(__fmaf_rn(s[kt][e], a.scale2, msafe[e >> 1]));
-          l[e >> 1] += p[kt][e];
-        }
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        // A fragments: a0 (row g, keys 0..7) a1 (row g+8) a2 (row g, keys 8..15) a3
-        uint32_t ph[4], pl[4];
+        if constexpr (BITS != 16) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          float sv[2] = {1.0f, 1.0f}, bv[2] = {0.0f, 0.0f};
-          if constexpr (BITS != 16) {
+          for (int kt = 0; kt < 2; ++kt) {
+            const float sv = half_bf(f.vs[kt], i);
+            const float bv = __fmaf_rn(BITS == 8 ? 128.0f : 8.0f, sv, half_bf(f.vb[kt], i));
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              sv[e] = pair_at<NG>(f.vs[kt], e, i);
-              bv[e] = __fmaf_rn(BITS == 8 ? 128.0f : 8.0f, sv[e], pair_at<NG>(f.vb[kt], e, i));
+            for (int nt = 0; nt < NT; ++nt) {
+              const float x0 = p[nt][2 * kt] * sv, x1 = p[nt][2 * kt + 1] * sv;
+              vbs[nt][0][i] = __fmaf_rn(p[nt][2 * kt], bv, vbs[nt][0][i]);
+              vbs[nt][1][i] = __fmaf_rn(p[nt][2 * kt + 1], bv, vbs[nt][1][i]);
+              const uint32_t hi = pk_bf2(x0, x1);
+              ph[nt][kt] = movm_t(hi);
+              pl[nt][kt] = movm_t(pk_bf2(x0 - lo_bf(hi), x1 - hi_bf(hi)));
             }
-          }
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float x0 = p[kt][2 * k], x1 = p[kt][2 * k + 1];
-            if constexpr (BITS != 16) {
-              vbs[k][i] = __fmaf_rn(x1, bv[1], __fmaf_rn(x0, bv[0], vbs[k][i]));
-              x0 *= sv[0];
-              x1 *= sv[1];
-            }
-            const uint32_t hi = pk_bf2(x0, x1);
-            ph[2 * kt + k] = hi;
-            pl[2 * kt + k] = pk_bf2(x0 - lo_bf(hi), x1 - hi_bf(hi));
           }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t vv[2];
+        for (int j = 0; j < 4; ++j) {
+          uint32_t vv[2][2];  // head dims 8g + j and 8g + j + 4; keys 2c, 2c + 1 and 2c + 8, 2c + 9
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if constexpr (BITS == 16) {
-              vv[k] = __byte_perm(f.v[2 * k][4 * i + j / 2], f.v[2 * k + 1][4 * i + j / 2], (j & 1) ? 0x7632 : 0x5410);
-            } else if constexpr (BITS == 8) {
-              vv[k] = code8_pair(__byte_perm(f.v[2 * k][2 * i + j / 4], f.v[2 * k + 1][2 * i + j / 4],
-                                             (j & 3) | ((4 + (j & 3)) << 8)));
-            } else {  // code - 8
-              const uint32_t t = __byte_perm(f.v[2 * k][i], f.v[2 * k + 1][i], j < 4 ? 0x5410 : 0x7632) >> (4 * (j & 3));
-              vv[k] = bf2_fma3((t & 0x000F000Fu) | 0x43004300u, 0x3F803F80u, 0xC308C308u);
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int d = j + 4 * u;
+              if constexpr (BITS == 16) {
+                vv[u][k] = __byte_perm(f.v[2 * k][4 * i + d / 2], f.v[2 * k + 1][4 * i + d / 2], (d & 1) ? 0x7632 : 0x5410);
+              } else if constexpr (BITS == 8) {
+                vv[u][k] = code8_pair(__byte_perm(f.v[2 * k][2 * i + u], f.v[2 * k + 1][2 * i + u], j | ((4 + j) << 8)));
+              } else {  // code - 8
+                const uint32_t t = __byte_perm(f.v[2 * k][i], f.v[2 * k + 1][i], u ? 0x7632 : 0x5410) >> (4 * j);
+                vv[u][k] = bf2_fma3((t & 0x000F000Fu) | 0x43004300u, 0x3F803F80u, 0xC308C308u);
+              }
             }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_bf16(o[nt][i][j], vv[0][0], vv[1][0], vv[0][1], vv[1][1], ph[nt][0], ph[nt][1]);
+            mma_bf16(o[nt][i][j], vv[0][0], vv[1][0], vv[0][1], vv[1][1], pl[nt][0], pl[nt][1]);
           }
-          mma_bf16(o[i][j], ph[0], ph[1], ph[2], ph[3], vv[0], vv[1]);
-          mma_bf16(o[i][j], pl[0], pl[1], pl[2], pl[3], vv[0], vv[1]);
         }
       }
       load_v(nrow, cnt);
@@ -926,46 +968,46 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
     // the four warps' results meet: sums over the lanes of a row, then
     // exp-weighted sums over the warps
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      l[k] = warp_sum_xor(l[k], 2, 1);
-      if constexpr (BITS != 16) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < NG; ++i) vbs[k][i] = warp_sum_xor(vbs[k][i], 2, 1);
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * nt + 2 * c + e;
+        l[nt][e] = warp_sum_xor(l[nt][e], 16, 4);
+        if (g == 0) {
+          sm_m[warp][r] = m[nt][e];
+          sm_l[warp][r] = l[nt][e];
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          float add = 0.0f;
+          if constexpr (BITS != 16) add = warp_sum_xor(vbs[nt][e][i], 16, 4);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<float4*>(&sm_o[warp][r][64 * i + 8 * g + 4 * u]) =
+                make_float4(o[nt][i][0][2 * u + e] + add, o[nt][i][1][2 * u + e] + add, o[nt][i][2][2 * u + e] + add,
+                            o[nt][i][3][2 * u + e] + add);
+        }
       }
-      if (c == 0) {
-        sm_m[warp][g + 8 * k] = m[k];
-        sm_l[warp][g + 8 * k] = l[k];
-      }
-      // lane (g, c) holds columns 64 i + 16 c .. + 15 of its rows
-#pragma unroll
-      for (int i = 0; i < NG; ++i)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int j = 0; j < 8; j += 4)
-            *reinterpret_cast<float4*>(&sm_o[warp][g + 8 * k][64 * i + 16 * c + 8 * half + j]) =
-                make_float4(o[i][j][2 * k + half] + vbs[k][i], o[i][j + 1][2 * k + half] + vbs[k][i],
-                            o[i][j + 2][2 * k + half] + vbs[k][i], o[i][j + 3][2 * k + half] + vbs[k][i]);
-    }
     __syncthreads();
     {
-      const int row16 = tid >> 3, col = (tid & 7) * (D / 8);
+      constexpr int TPR = 128 / R, W = D / TPR;  // threads of a row, columns of a thread
+      const int row = tid / TPR, col = tid % TPR * W;
       float M = -INFINITY, L = 0.0f, w[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) M = fmaxf(M, sm_m[k][row16]);
+      for (int k = 0; k < 4; ++k) M = fmaxf(M, sm_m[k][row]);
       const float ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        w[k] = ex2f(sm_m[k][row16] - ms);
-        L = __fmaf_rn(w[k], sm_l[k][row16], L);
+        w[k] = ex2f(sm_m[k][row] - ms);
+        L = __fmaf_rn(w[k], sm_l[k][row], L);
       }
-      float acc[D / 8];
+      float acc[W];
 #pragma unroll
-      for (int d = 0; d < D / 8; d += 4) {
+      for (int d = 0; d < W; d += 4) {
         float4 s4 = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float4 x = *reinterpret_cast<const float4*>(&sm_o[k][row16][col + d]);
+          const float4 x = *reinterpret_cast<const float4*>(&sm_o[k][row][col + d]);
           s4.x = __fmaf_rn(w[k], x.x, s4.x);
           s4.y = __fmaf_rn(w[k], x.y, s4.y);
           s4.z = __fmaf_rn(w[k], x.z, s4.z);
@@ -973,28 +1015,25 @@ __global__ void __launch_bounds__(128, D == 64 ? 3 : 2) paged_attn_kernel(PagedA
         }
         acc[d] = s4.x; acc[d + 1] = s4.y; acc[d + 2] = s4.z; acc[d + 3] = s4.w;
       }
-      const int r = tile * 16 + row16, t = r / a.G;
+      const int r = tile * R + row, t = r / a.G;
       if (t < z.nnew) {
         if (b0 == 0 && b1 == z.nblk) {
           const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
           const int head = h * a.G + r % a.G;
           bf16_t* op = a.out + (int64_t)(z.first + t) * a.ldo + (int64_t)head * D + col;
 #pragma unroll
-          for (int d = 0; d < D / 8; d += 8) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = acc[d + e] * inv;
-            *reinterpret_cast<uint4*>(op + d) = bf8_pack(y);
-          }
-          if (a.lse && (tid & 7) == 0)
+          for (int d = 0; d < W; d += 4)
+            *reinterpret_cast<uint2*>(op + d) =
+                make_uint2(pk_bf2(acc[d] * inv, acc[d + 1] * inv), pk_bf2(acc[d + 2] * inv, acc[d + 3] * inv));
+          if (a.lse && tid % TPR == 0)
             a.lse[(int64_t)(z.first + t) * a.heads + head] =
                 L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
         } else {
           const int64_t slot = 2 * (int64_t)blockIdx.x + (first_seg ? 0 : 1);
-          float* pp = a.part + (slot * 16 + row16) * D + col;
+          float* pp = a.part + (slot * R + row) * D + col;
 #pragma unroll
-          for (int d = 0; d < D / 8; d += 4) *reinterpret_cast<float4*>(pp + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
-          if ((tid & 7) == 0) *reinterpret_cast<float2*>(a.ml + (slot * 16 + row16) * 2) = make_float2(M, L);
+          for (int d = 0; d < W; d += 4) *reinterpret_cast<float4*>(pp + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+          if (tid % TPR == 0) *reinterpret_cast<float2*>(a.ml + (slot * R + row) * 2) = make_float2(M, L);
         }
       }
     }
@@ -1021,7 +1060,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(PagedAttnArgs a) {
   const PagedSpan z = paged_span(a, seq);
   const int h = head / a.G, r = (t - z.first) * a.G + head % a.G;
   const int64_t total = a.prefix[a.b.seqs], n = total < a.nctas ? total : a.nctas;
-  const int64_t i0 = a.prefix[seq] + ((int64_t)h * z.tiles + r / 16) * z.nblk, i1 = i0 + z.nblk;
+  const int64_t i0 = a.prefix[seq] + ((int64_t)h * z.tiles + r / a.rows) * z.nblk, i1 = i0 + z.nblk;
   // CTA c owns blocks [total*c/n, total*(c+1)/n)
   const int c0 = (int)(((i0 + 1) * n - 1) / total), c1 = (int)((i1 * n - 1) / total);
   if (c0 == c1) return;  // written by its CTA
@@ -1029,7 +1068,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(PagedAttnArgs a) {
   float M = -INFINITY, L = 0.0f, acc[V] = {};
 #pragma unroll 4
   for (int k = c0 + warp; k <= c1; k += 4) {
-    const int64_t s = (int64_t)(k == c0 ? slot0 : 2 * k) * 16 + r % 16;
+    const int64_t s = (int64_t)(k == c0 ? slot0 : 2 * k) * a.rows + r % a.rows;
     const float2 ml = *reinterpret_cast<const float2*>(a.ml + s * 2);
     float x[V];
 #pragma unroll

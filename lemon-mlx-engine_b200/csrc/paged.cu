@@ -305,8 +305,8 @@ int check_attn(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads, 
   }
   if (rc) return rc;
   auto after = [](size_t at, size_t bytes) { return (at + bytes + 255) / 256 * 256; };
-  p.start = after(0, (size_t)(batch->seqs + 1) * 8);
-  p.ml = after(p.start, p.prompt ? (size_t)p.nctas * sizeof(int4) : 0);
+  p.start = 256;  // behind the total
+  p.ml = after(p.start, (p.prompt ? (size_t)p.nctas : (size_t)batch->tokens * heads) * sizeof(int4));
   p.part = after(p.ml, (size_t)2 * p.nctas * p.rows * 2 * 4);
   p.bytes = p.part + (size_t)2 * p.nctas * p.rows * D * 4;
   return LMX_OK;
@@ -377,7 +377,8 @@ int launch_prompt(const PagedAttnArgs& a, const AttnPlan& pl, cudaStream_t st) {
 }
 
 template <int D, int BITS, int NT>
-int launch_few(const PagedAttnArgs& a, cudaStream_t st) {
+int launch_few(PagedAttnArgs a, cudaStream_t st) {
+  a.keys = PagedStep<D, BITS, NT>::KEYS;
   int rc = cuda_check(lmx_launch(paged_attn_kernel<D, BITS, NT>, dim3(a.nctas), dim3(128), (size_t)(a.b.seqs + 1) * 8, st, true, a),
                       "paged_attention: launch");
   if (rc) return rc;
@@ -434,7 +435,9 @@ extern "C" int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch
   a.ml = (float*)((uint8_t*)scratch + p.ml);
   a.part = (float*)((uint8_t*)scratch + p.part);
   a.rows = p.rows;
+  a.shared_by = (int4*)((uint8_t*)scratch + p.start);
   a.nctas = p.nctas;
+  a.sms = device_sms();
   a.err = device_error_word();
   cudaStream_t st = (cudaStream_t)stream;
   if (p.prompt) {

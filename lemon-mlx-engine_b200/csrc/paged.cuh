@@ -468,7 +468,17 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
 // z = 8 or 128 being the middle of the code range, so that the first sum
 // does not cancel against the second.
 // ---------------------------------------------------------------------------
-static constexpr int kPagedKeys = 64;  // keys per block
+// Shape of the few-row kernel.  KP: 16-key groups that a warp takes at a time;
+// two share a maximum, a rescale and the index work (64-wide 4-bit heads, 16 x
+// 8000 rows: 44.7 -> 39.7 us), but for 128-wide ones they spill (8-bit: 63 -> 73 us).
+// CTAS per SM: with eight rows the registers allow three (8-bit: two take 85 us,
+// three 65), with four they spill (79); 16 rows hold twice the accumulators.
+template <int D, int BITS, int NT>
+struct PagedStep {
+  static constexpr int KP = BITS != 16 && D == 64 ? 2 : 1;
+  static constexpr int CTAS = NT == 1 || D == 64 ? 3 : 2;
+  static constexpr int KEYS = 64 * KP;  // per block (four warps)
+};
 
 struct PagedAttnArgs {
   PagedKv kv;
@@ -481,11 +491,14 @@ struct PagedAttnArgs {
   bf16_t* out;
   int64_t ldo;
   float* lse;
-  int64_t* prefix;  // scratch: blocks before each sequence [seqs + 1]
+  int64_t* prefix;  // scratch (prompt kernel): total blocks
   float* ml;        // [2 * grid][rows][2]
   float* part;      // [2 * grid][rows][D]
   int rows;         // query rows of a tile (few-row kernel: 8 or 16)
-  int nctas;
+  int keys;         // keys of a block (few-row kernel)
+  int4* shared_by;  // [tokens * heads] of a row: its item's first CTA (-1: one CTA has all
+                    // of it), last CTA, first slot, row in the tile
+  int nctas, sms;
   unsigned* err;
 };
 
@@ -504,11 +517,27 @@ LMX_DEV PagedSpan paged_span(const PagedAttnArgs& a, int s) {
   z.lo = 0;
   if (a.window > 0) z.lo = max(0, __ldg(a.b.kv_len + s) - z.nnew - a.window + 1) & ~15;
   z.tiles = (int)(((int64_t)z.nnew * a.G + a.rows - 1) / a.rows);
-  z.nblk = max(1, (max(z.len - z.lo, 0) + kPagedKeys - 1) / kPagedKeys);
+  z.nblk = max(1, (max(z.len - z.lo, 0) + a.keys - 1) / a.keys);
   return z;
 }
 LMX_DEV int64_t paged_span_blocks(const PagedAttnArgs& a, const PagedSpan& z) {
   return (int64_t)z.tiles * z.nblk * a.kv.Hk;
+}
+
+// where CTA c of n begins in `total` blocks (32-bit arithmetic where it does)
+LMX_DEV int64_t paged_share(int64_t total, int64_t c, int64_t n) {
+  return total < (1 << 20) ? (int64_t)((uint32_t)total * (uint32_t)c / (uint32_t)n) : total * c / n;
+}
+// the CTA that has block i
+LMX_DEV int paged_owner(int64_t total, int64_t i, int64_t n) {
+  return (int)(total < (1 << 20) ? (int64_t)(((uint32_t)(i + 1) * (uint32_t)n - 1) / (uint32_t)total) : ((i + 1) * n - 1) / total);
+}
+// CTAs that share `total` blocks: each block its own while the SMs last, then
+// four blocks each until the wave is full, because every CTA leaves a partial
+// result to join (1 x 8000 rows, 64 heads: 21.2 us with one block each, 18.0
+// with four; 1 x 700 rows, 16 heads: 8.3 against 11.6)
+LMX_DEV int64_t paged_ctas(int64_t total, int nctas, int sms) {
+  return total <= sms ? total : min((int64_t)nctas, max((int64_t)sms, total / 4));
 }
 
 // blocks before each sequence, by the whole CTA (128 threads) into shared memory
@@ -636,15 +665,13 @@ LMX_DEV uint32_t movm_t(uint32_t x) {
 }
 LMX_DEV float half_bf(uint32_t w, int i) { return i ? hi_bf(w) : lo_bf(w); }
 
-#ifndef FEWCTA
-#define FEWCTA 3
-#endif
 // NT: 8-row tiles of query rows
 template <int D, int BITS, int NT>
-__global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) paged_attn_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(128, PagedStep<D, BITS, NT>::CTAS) paged_attn_kernel(PagedAttnArgs a) {
   using F = PagedFrag<D, BITS>;
   constexpr int NG = D / 64, QW = D / 8;  // Q words per lane and row
   constexpr int R = 8 * NT, OP = D + 4;   // rows, pitch of the merge buffer
+  constexpr int KP = PagedStep<D, BITS, NT>::KP;  // 16-key groups per step
   extern __shared__ int64_t pre[];
   __shared__ int64_t wsum[4];
   __shared__ float sm_m[4][R], sm_l[4][R];
@@ -656,16 +683,15 @@ __global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) pag
   paged_prefix(a, pre, wsum);
   const int64_t total = pre[a.b.seqs];
   if (blockIdx.x == 0) {
-    for (int s = tid; s <= a.b.seqs; s += 128) a.prefix[s] = pre[s];
     for (int s = tid; s < a.b.seqs; s += 128)
       if (__ldg(a.b.kv_len + s) > ((int64_t)a.b.table_stride << a.kv.logP) &&
           __ldg(a.b.q_start + s + 1) > __ldg(a.b.q_start + s))
         atomicExch(a.err, kPagedErr);
   }
-  const int64_t n = total < a.nctas ? total : a.nctas;
+  const int64_t n = paged_ctas(total, a.nctas, a.sms);
   if (blockIdx.x >= n) return;
-  int64_t at = total * blockIdx.x / n;
-  const int64_t end = total * (blockIdx.x + 1) / n;
+  int64_t at = paged_share(total, blockIdx.x, n);
+  const int64_t end = paged_share(total, blockIdx.x + 1, n);
   int seq = 0;
   {
     int hi = a.b.seqs;  // last sequence whose prefix is <= at
@@ -680,7 +706,13 @@ __global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) pag
     while (pre[seq + 1] <= at) ++seq;
     const PagedSpan z = paged_span(a, seq);
     const int64_t loc = at - pre[seq];
-    const int b0 = (int)(loc % z.nblk), tile = (int)(loc / z.nblk % z.tiles), h = (int)(loc / z.nblk / z.tiles);
+    int b0, tile, h;
+    if (loc < (1ll << 31)) {
+      const uint32_t x = (uint32_t)loc / (uint32_t)z.nblk;
+      b0 = (int)((uint32_t)loc % (uint32_t)z.nblk), tile = (int)(x % (uint32_t)z.tiles), h = (int)(x / (uint32_t)z.tiles);
+    } else {
+      b0 = (int)(loc % z.nblk), tile = (int)(loc / z.nblk % z.tiles), h = (int)(loc / z.nblk / z.tiles);
+    }
     const int b1 = (int)min((int64_t)z.nblk, b0 + (end - at));
 
     // a lane's query fragments are of rows 8 nt + g, its scores of rows 8 nt + 2c, + 1
@@ -771,102 +803,111 @@ __global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) pag
         l[nt][e] = 0.0f;
       }
 
-    // step b: keys [lo + 64 b + 16 warp, +16); its row of head h, or -1
-    auto row_of = [&](int b, int& cnt) -> int64_t {
-      const int key = z.lo + b * kPagedKeys + warp * 16;
+    // step b, group kp: 16 keys from lo + 64 KP b + 16 (KP warp + kp); their row of head h, or -1
+    auto row_of = [&](int b, int kp, int& cnt) -> int64_t {
+      const int key = z.lo + b * (64 * KP) + (warp * KP + kp) * 16;
       cnt = z.len - key;
       if (b >= b1 || cnt <= 0) return -1;
       const int64_t r = paged_row(a.kv, a.b, seq, key);
       if (r < 0 && lane == 0) atomicExch(a.err, kPagedErr);
       return r < 0 ? -1 : r + (int64_t)h * a.kv.P;
     };
-    F f;
-    auto load_k = [&](int64_t row, int cnt) {
-      if (cnt >= 16 && row >= 0) paged_load_k<D, BITS, true>(f, a.kv, row, cnt, g, c);
-      else paged_load_k<D, BITS, false>(f, a.kv, row, cnt, g, c);
+    F f[KP];
+    auto load_k = [&](int kp, int64_t row, int cnt) {
+      if (cnt >= 16 && row >= 0) paged_load_k<D, BITS, true>(f[kp], a.kv, row, cnt, g, c);
+      else paged_load_k<D, BITS, false>(f[kp], a.kv, row, cnt, g, c);
     };
-    auto load_v = [&](int64_t row, int cnt) {
-      if (cnt >= 16 && row >= 0) paged_load_v<D, BITS, true>(f, a.kv, row, cnt, g, c);
-      else paged_load_v<D, BITS, false>(f, a.kv, row, cnt, g, c);
+    auto load_v = [&](int kp, int64_t row, int cnt) {
+      if (cnt >= 16 && row >= 0) paged_load_v<D, BITS, true>(f[kp], a.kv, row, cnt, g, c);
+      else paged_load_v<D, BITS, false>(f[kp], a.kv, row, cnt, g, c);
     };
-    int cnt;
-    {
-      const int64_t row = row_of(b0, cnt);
-      load_k(row, cnt);
-      load_v(row, cnt);
+    int cnt[KP];
+    int64_t nrow[KP];
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      nrow[kp] = row_of(b0, kp, cnt[kp]);
+      load_k(kp, nrow[kp], cnt[kp]);
     }
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) load_v(kp, nrow[kp], cnt[kp]);
     for (int b = b0; b < b1; ++b) {
-      const int64_t nrow = row_of(b + 1, cnt);
-      // s[nt]: key g rows 2c, 2c + 1, then key g + 8
-      float s[NT][4];
-      if constexpr (BITS == 16) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+      for (int kp = 0; kp < KP; ++kp) nrow[kp] = row_of(b + 1, kp, cnt[kp]);
+      float sk[KP][NT][4];
 #pragma unroll
-          for (int w = 0; w < QW; w += 2)
-            mma_bf16(s[nt], f.k[0][w], f.k[1][w], f.k[0][w + 1], f.k[1][w + 1], qf[nt][w], qf[nt][w + 1]);
-        }
-      } else {
-        float sg[NT][NG][4] = {};
+      for (int kp = 0; kp < KP; ++kp) {
+        const F& fk = f[kp];
+        float(&s)[NT][4] = sk[kp];
+        // s[nt]: key g rows 2c, 2c + 1, then key g + 8
+        if constexpr (BITS == 16) {
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
+          for (int nt = 0; nt < NT; ++nt) {
+            s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {  // k16 steps of the group
-            uint32_t k0[2], k1[2];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-              if constexpr (BITS == 8) {  // exact fp16 1024 + code
-                const uint32_t x = f.k[kt][4 * i + j];
-                k0[kt] = __byte_perm(x, 0x64646464u, 0x4140);
-                k1[kt] = __byte_perm(x, 0x64646464u, 0x4342);
-              } else {  // exact bf16 128 + code
-                const uint32_t x = f.k[kt][2 * i + (j >> 1)] >> (8 * (j & 1));
-                k0[kt] = (x & 0x000F000Fu) | 0x43004300u;
-                k1[kt] = ((x >> 4) & 0x000F000Fu) | 0x43004300u;
-              }
-            }
-            const int w = 8 * i + 2 * j;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if constexpr (BITS == 8) mma_f16(sg[nt][i], k0[0], k0[1], k1[0], k1[1], qf[nt][w], qf[nt][w + 1]);
-              else mma_bf16(sg[nt][i], k0[0], k0[1], k1[0], k1[1], qf[nt][w], qf[nt][w + 1]);
-            }
+            for (int w = 0; w < QW; w += 2)
+              mma_bf16(s[nt], fk.k[0][w], fk.k[1][w], fk.k[0][w + 1], fk.k[1][w + 1], qf[nt][w], qf[nt][w + 1]);
           }
-        }
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          float sc[NG], bi[NG];
+        } else {
+          float sg[NT][NG][4] = {};
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
-            sc[i] = half_bf(f.ks[kt], i);
-            bi[i] = __fmaf_rn(BITS == 8 ? -1024.0f : -128.0f, sc[i], half_bf(f.kb[kt], i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // k16 steps of the group
+              uint32_t k0[2], k1[2];
+#pragma unroll
+              for (int kt = 0; kt < 2; ++kt) {
+                if constexpr (BITS == 8) {  // exact fp16 1024 + code
+                  const uint32_t x = fk.k[kt][4 * i + j];
+                  k0[kt] = __byte_perm(x, 0x64646464u, 0x4140);
+                  k1[kt] = __byte_perm(x, 0x64646464u, 0x4342);
+                } else {  // exact bf16 128 + code
+                  const uint32_t x = fk.k[kt][2 * i + (j >> 1)] >> (8 * (j & 1));
+                  k0[kt] = (x & 0x000F000Fu) | 0x43004300u;
+                  k1[kt] = ((x >> 4) & 0x000F000Fu) | 0x43004300u;
+                }
+              }
+              const int w = 8 * i + 2 * j;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if constexpr (BITS == 8) mma_f16(sg[nt][i], k0[0], k0[1], k1[0], k1[1], qf[nt][w], qf[nt][w + 1]);
+                else mma_bf16(sg[nt][i], k0[0], k0[1], k1[0], k1[1], qf[nt][w], qf[nt][w + 1]);
+              }
+            }
           }
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            float sc[NG], bi[NG];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+              sc[i] = half_bf(fk.ks[kt], i);
+              bi[i] = __fmaf_rn(BITS == 8 ? -1024.0f : -128.0f, sc[i], half_bf(fk.kb[kt], i));
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float x = bi[0] * qs[nt][e][0];
+#pragma unroll
+                for (int i = 1; i < NG; ++i) x = __fmaf_rn(bi[i], qs[nt][e][i], x);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) x = __fmaf_rn(sc[i], sg[nt][i][2 * kt + e], x);
+                s[nt][2 * kt + e] = x;
+              }
+          }
+        }
+        load_k(kp, nrow[kp], cnt[kp]);
+
+        // keys a row does not see at -infinity
+        const int key = z.lo + b * (64 * KP) + (warp * KP + kp) * 16;
+        if (key + 16 > all_hi || key < all_lo) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = bi[0] * qs[nt][e][0];
-#pragma unroll
-              for (int i = 1; i < NG; ++i) x = __fmaf_rn(bi[i], qs[nt][e][i], x);
-#pragma unroll
-              for (int i = 0; i < NG; ++i) x = __fmaf_rn(sc[i], sg[nt][i][2 * kt + e], x);
-              s[nt][2 * kt + e] = x;
+            for (int e = 0; e < 4; ++e) {
+              const int j = key + g + 8 * (e >> 1);
+              if (j >= khi[nt][e & 1] || j < klo[nt][e & 1]) s[nt][e] = -INFINITY;
             }
         }
-      }
-      load_k(nrow, cnt);
-
-      // keys a row does not see at -infinity
-      const int key = z.lo + b * kPagedKeys + warp * 16;
-      if (key + 16 > all_hi || key < all_lo) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = key + g + 8 * (e >> 1);
-            if (j >= khi[nt][e & 1] || j < klo[nt][e & 1]) s[nt][e] = -INFINITY;
-          }
       }
       float mn[NT][2];
       bool grow = false;
@@ -874,7 +915,9 @@ __global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) pag
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+          float mx = fmaxf(sk[0][nt][e], sk[0][nt][2 + e]);
+#pragma unroll
+          for (int kp = 1; kp < KP; ++kp) mx = fmaxf(mx, fmaxf(sk[kp][nt][e], sk[kp][nt][2 + e]));
 #pragma unroll
           for (int off = 4; off <= 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
           mx *= a.scale2;
@@ -900,69 +943,73 @@ __global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) pag
             }
           }
       }
-      // p, and (bf16 caches) its two terms as P^T's fragments
-      float p[NT][4];
-      uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int kp = 0; kp < KP; ++kp) {
+        const F& fk = f[kp];
+        // p, and (bf16 caches) its two terms as P^T's fragments
+        float p[NT][4];
+        uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float ms = m[nt][e & 1] == -INFINITY ? 0.0f : -m[nt][e & 1];
-          p[nt][e] = ex2f(__fmaf_rn(s[nt][e], a.scale2, ms));
-          l[nt][e & 1] += p[nt][e];
-        }
-        if constexpr (BITS == 16) {
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            const uint32_t hi = pk_bf2(p[nt][2 * kt], p[nt][2 * kt + 1]);
-            ph[nt][kt] = movm_t(hi);
-            pl[nt][kt] = movm_t(pk_bf2(p[nt][2 * kt] - lo_bf(hi), p[nt][2 * kt + 1] - hi_bf(hi)));
+          for (int e = 0; e < 4; ++e) {
+            const float ms = m[nt][e & 1] == -INFINITY ? 0.0f : -m[nt][e & 1];
+            p[nt][e] = ex2f(__fmaf_rn(sk[kp][nt][e], a.scale2, ms));
+            l[nt][e & 1] += p[nt][e];
           }
-        }
-      }
+          if constexpr (BITS == 16) {
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        if constexpr (BITS != 16) {
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            const float sv = half_bf(f.vs[kt], i);
-            const float bv = __fmaf_rn(BITS == 8 ? 128.0f : 8.0f, sv, half_bf(f.vb[kt], i));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float x0 = p[nt][2 * kt] * sv, x1 = p[nt][2 * kt + 1] * sv;
-              vbs[nt][0][i] = __fmaf_rn(p[nt][2 * kt], bv, vbs[nt][0][i]);
-              vbs[nt][1][i] = __fmaf_rn(p[nt][2 * kt + 1], bv, vbs[nt][1][i]);
-              const uint32_t hi = pk_bf2(x0, x1);
+            for (int kt = 0; kt < 2; ++kt) {
+              const uint32_t hi = pk_bf2(p[nt][2 * kt], p[nt][2 * kt + 1]);
               ph[nt][kt] = movm_t(hi);
-              pl[nt][kt] = movm_t(pk_bf2(x0 - lo_bf(hi), x1 - hi_bf(hi)));
+              pl[nt][kt] = movm_t(pk_bf2(p[nt][2 * kt] - lo_bf(hi), p[nt][2 * kt + 1] - hi_bf(hi)));
             }
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t vv[2][2];  // head dims 8g + j and 8g + j + 4; keys 2c, 2c + 1 and 2c + 8, 2c + 9
+        for (int i = 0; i < NG; ++i) {
+          if constexpr (BITS != 16) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+            for (int kt = 0; kt < 2; ++kt) {
+              const float sv = half_bf(fk.vs[kt], i);
+              const float bv = __fmaf_rn(BITS == 8 ? 128.0f : 8.0f, sv, half_bf(fk.vb[kt], i));
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int d = j + 4 * u;
-              if constexpr (BITS == 16) {
-                vv[u][k] = __byte_perm(f.v[2 * k][4 * i + d / 2], f.v[2 * k + 1][4 * i + d / 2], (d & 1) ? 0x7632 : 0x5410);
-              } else if constexpr (BITS == 8) {
-                vv[u][k] = code8_pair(__byte_perm(f.v[2 * k][2 * i + u], f.v[2 * k + 1][2 * i + u], j | ((4 + j) << 8)));
-              } else {  // code - 8
-                const uint32_t t = __byte_perm(f.v[2 * k][i], f.v[2 * k + 1][i], u ? 0x7632 : 0x5410) >> (4 * j);
-                vv[u][k] = bf2_fma3((t & 0x000F000Fu) | 0x43004300u, 0x3F803F80u, 0xC308C308u);
+              for (int nt = 0; nt < NT; ++nt) {
+                const float x0 = p[nt][2 * kt] * sv, x1 = p[nt][2 * kt + 1] * sv;
+                vbs[nt][0][i] = __fmaf_rn(p[nt][2 * kt], bv, vbs[nt][0][i]);
+                vbs[nt][1][i] = __fmaf_rn(p[nt][2 * kt + 1], bv, vbs[nt][1][i]);
+                const uint32_t hi = pk_bf2(x0, x1);
+                ph[nt][kt] = movm_t(hi);
+                pl[nt][kt] = movm_t(pk_bf2(x0 - lo_bf(hi), x1 - hi_bf(hi)));
               }
             }
+          }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_bf16(o[nt][i][j], vv[0][0], vv[1][0], vv[0][1], vv[1][1], ph[nt][0], ph[nt][1]);
-            mma_bf16(o[nt][i][j], vv[0][0], vv[1][0], vv[0][1], vv[1][1], pl[nt][0], pl[nt][1]);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t vv[2][2];  // head dims 8g + j and 8g + j + 4; keys 2c, 2c + 1 and 2c + 8, 2c + 9
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int d = j + 4 * u;
+                if constexpr (BITS == 16) {
+                  vv[u][k] = __byte_perm(fk.v[2 * k][4 * i + d / 2], fk.v[2 * k + 1][4 * i + d / 2], (d & 1) ? 0x7632 : 0x5410);
+                } else if constexpr (BITS == 8) {
+                  vv[u][k] = code8_pair(__byte_perm(fk.v[2 * k][2 * i + u], fk.v[2 * k + 1][2 * i + u], j | ((4 + j) << 8)));
+                } else {  // code - 8
+                  const uint32_t t = __byte_perm(fk.v[2 * k][i], fk.v[2 * k + 1][i], u ? 0x7632 : 0x5410) >> (4 * j);
+                  vv[u][k] = bf2_fma3((t & 0x000F000Fu) | 0x43004300u, 0x3F803F80u, 0xC308C308u);
+                }
+              }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_bf16(o[nt][i][j], vv[0][0], vv[1][0], vv[0][1], vv[1][1], ph[nt][0], ph[nt][1]);
+              mma_bf16(o[nt][i][j], vv[0][0], vv[1][0], vv[0][1], vv[1][1], pl[nt][0], pl[nt][1]);
+            }
           }
         }
+        load_v(kp, nrow[kp], cnt[kp]);
       }
-      load_v(nrow, cnt);
     }
 
     // the four warps' results meet: sums over the lanes of a row, then
@@ -1017,6 +1064,16 @@ __global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) pag
       }
       const int r = tile * R + row, t = r / a.G;
       if (t < z.nnew) {
+        if (b1 == z.nblk && tid % TPR == 0) {  // the item's last CTA says who shares it
+          const int64_t i0 = at - b0;
+          int4 by = make_int4(-1, 0, 0, row);
+          if (b0 > 0) {
+            by.x = paged_owner(total, i0, n);
+            by.y = (int)blockIdx.x;
+            by.z = 2 * by.x + (paged_share(total, by.x, n) < i0 ? 1 : 0);
+          }
+          a.shared_by[(int64_t)(z.first + t) * a.heads + h * a.G + r % a.G] = by;
+        }
         if (b0 == 0 && b1 == z.nblk) {
           const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
           const int head = h * a.G + r % a.G;
@@ -1044,9 +1101,9 @@ __global__ void __launch_bounds__(128, NT == 1 ? FEWCTA : (D == 64 ? 3 : 2)) pag
 }
 
 // Join of the items that several CTAs share: a CTA per (token, head), its four
-// warps taking every fourth contributor.  The contributors of blocks [i0, i1)
-// are CTAs c0 .. c1; only c0 can have begun in an earlier item (its slot 1),
-// the others begin inside this one.
+// warps taking every fourth contributor.  Only an item's first CTA can have
+// begun in an earlier item (its partial is then in its slot 1); the others
+// begin inside it.
 template <int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(PagedAttnArgs a) {
   constexpr int V = D / 32;
@@ -1055,20 +1112,14 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(PagedAttnArgs a) {
   grid_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = (int)(blockIdx.x / a.heads), head = (int)(blockIdx.x % a.heads);
-  const int seq = paged_seq(a.b, t, lane);
-  if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;
-  const PagedSpan z = paged_span(a, seq);
-  const int h = head / a.G, r = (t - z.first) * a.G + head % a.G;
-  const int64_t total = a.prefix[a.b.seqs], n = total < a.nctas ? total : a.nctas;
-  const int64_t i0 = a.prefix[seq] + ((int64_t)h * z.tiles + r / a.rows) * z.nblk, i1 = i0 + z.nblk;
-  // CTA c owns blocks [total*c/n, total*(c+1)/n)
-  const int c0 = (int)(((i0 + 1) * n - 1) / total), c1 = (int)((i1 * n - 1) / total);
-  if (c0 == c1) return;  // written by its CTA
-  const int slot0 = 2 * c0 + (total * c0 / n < i0 ? 1 : 0);
+  const int4 by = a.shared_by[blockIdx.x];
+  const int32_t q0 = __ldg(a.b.q_start), q1 = __ldg(a.b.q_start + a.b.seqs);
+  if (t < q0 || t >= q1 || by.x < 0) return;  // padding, or written by its CTA
+  const int c0 = by.x, c1 = by.y, slot0 = by.z, row = by.w;
   float M = -INFINITY, L = 0.0f, acc[V] = {};
 #pragma unroll 4
   for (int k = c0 + warp; k <= c1; k += 4) {
-    const int64_t s = (int64_t)(k == c0 ? slot0 : 2 * k) * a.rows + r % a.rows;
+    const int64_t s = (int64_t)(k == c0 ? slot0 : 2 * k) * a.rows + row;
     const float2 ml = *reinterpret_cast<const float2*>(a.ml + s * 2);
     float x[V];
 #pragma unroll

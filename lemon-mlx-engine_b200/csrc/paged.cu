@@ -1,5 +1,6 @@
 // paged.cu -- host launchers and C ABI of the rotary and paged-cache
 // operators (include/lmx.h, "Paged KV cache").
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <type_traits>
@@ -87,6 +88,28 @@ int check_rope(const lmx_rope* r, int head_dim, const char* who) {
 
 // token rows of `heads` heads, ld values apart
 bool bad_rows(const void* p, int64_t ld, int64_t width) { return !p || !aligned16(p) || ld < width || ld % 8; }
+
+// f(head dim, bits) as compile-time constants
+template <typename F>
+auto on_cache(int D, int bits, F f) {
+  auto on_bits = [&](auto d) {
+    return bits == 16  ? f(d, std::integral_constant<int, 16>())
+           : bits == 8 ? f(d, std::integral_constant<int, 8>())
+                       : f(d, std::integral_constant<int, 4>());
+  };
+  return D == 64 ? on_bits(std::integral_constant<int, 64>()) : on_bits(std::integral_constant<int, 128>());
+}
+
+// A token's `steps` split over wpt warps of `run` steps: one warp a step while
+// that is at most RUNW warps per SM, longer runs beyond.
+#ifndef RUNW
+#define RUNW 64
+#endif
+void warp_runs(int tokens, int steps, int& run, int& wpt) {
+  const int64_t warps = (int64_t)device_sms() * RUNW;
+  run = (int)std::min<int64_t>(steps, std::max<int64_t>(1, (int64_t)tokens * steps / warps));
+  wpt = (steps + run - 1) / run;
+}
 
 int grid_of(int64_t blocks, unsigned& grid, const char* who) {
   if (blocks > 0x7fffffff) return set_error(LMX_ERR_UNSUPPORTED, "%s: too many rows", who);
@@ -208,14 +231,15 @@ extern "C" int lmx_paged_append(const lmx_paged_kv* kv, const lmx_paged_batch* b
   a.q_out = (bf16_t*)q_out;
   a.ldqo = ldq_out;
   a.err = device_error_word();
-  const int nh = heads + 2 * kv->kv_heads, it = 4, per = 256 / D * it;
-  const int64_t warps = (int64_t)batch->tokens * ((nh + per - 1) / per);
+  const int steps = (heads + 2 * kv->kv_heads + 512 / D - 1) / (512 / D);
+  warp_runs(batch->tokens, steps, a.run, a.wpt);
   unsigned grid;
-  if ((rc = grid_of((warps + 3) / 4, grid, "paged_append"))) return rc;
-  cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e = D == 64 ? lmx_launch(paged_append_kernel<64, it>, dim3(grid), dim3(128), 0, st, true, a)
-                          : lmx_launch(paged_append_kernel<128, it>, dim3(grid), dim3(128), 0, st, true, a);
-  return cuda_check(e, "paged_append: launch");
+  if ((rc = grid_of(((int64_t)batch->tokens * a.wpt + 3) / 4, grid, "paged_append"))) return rc;
+  return cuda_check(on_cache(D, kv->bits, [&](auto d, auto bits) {
+                      return lmx_launch(paged_append_kernel<decltype(d)::value, decltype(bits)::value>, dim3(grid),
+                                        dim3(128), 0, (cudaStream_t)stream, true, a);
+                    }),
+                    "paged_append: launch");
 }
 
 extern "C" int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* batch, void* k_out, void* v_out,
@@ -226,11 +250,14 @@ extern "C" int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* b
   if (!aligned16(k_out) || !aligned16(v_out))
     return set_error(LMX_ERR_INVALID, "paged_gather: k_out and v_out must be 16-byte aligned");
   if (batch->tokens == 0 || batch->seqs == 0 || (!k_out && !v_out)) return LMX_OK;
-  GatherArgs a{dev_kv(*kv), dev_batch(*batch), (bf16_t*)k_out, (bf16_t*)v_out, device_error_word()};
-  const dim3 grid((unsigned)(((int64_t)batch->tokens + 3) / 4));
-  cudaStream_t st = (cudaStream_t)stream;
-  return cuda_check(kv->head_dim == 64 ? lmx_launch(paged_gather_kernel<64>, grid, dim3(128), 0, st, true, a)
-                                       : lmx_launch(paged_gather_kernel<128>, grid, dim3(128), 0, st, true, a),
+  GatherArgs a{dev_kv(*kv), dev_batch(*batch), (bf16_t*)k_out, (bf16_t*)v_out, 0, 0, device_error_word()};
+  warp_runs(batch->tokens, (2 * kv->kv_heads * kv->head_dim / 8 + 31) / 32, a.run, a.wpt);
+  unsigned grid;
+  if ((rc = grid_of(((int64_t)batch->tokens * a.wpt + 3) / 4, grid, "paged_gather"))) return rc;
+  return cuda_check(on_cache(kv->head_dim, kv->bits, [&](auto d, auto bits) {
+                      return lmx_launch(paged_gather_kernel<decltype(d)::value, decltype(bits)::value>, dim3(grid),
+                                        dim3(128), 0, (cudaStream_t)stream, true, a);
+                    }),
                     "paged_gather: launch");
 }
 
@@ -273,15 +300,9 @@ int few_rows_ctas(int* n) {
 // f(head dim, bits, 8-row tiles) as compile-time constants
 template <typename F>
 int few_rows(int D, int bits, int rows, F f) {
-  auto nt = [&](auto d, auto b) {
+  return on_cache(D, bits, [&](auto d, auto b) {
     return rows == 8 ? f(d, b, std::integral_constant<int, 1>()) : f(d, b, std::integral_constant<int, 2>());
-  };
-  auto on_bits = [&](auto d) {
-    return bits == 16  ? nt(d, std::integral_constant<int, 16>())
-           : bits == 8 ? nt(d, std::integral_constant<int, 8>())
-                       : nt(d, std::integral_constant<int, 4>());
-  };
-  return D == 64 ? on_bits(std::integral_constant<int, 64>()) : on_bits(std::integral_constant<int, 128>());
+  });
 }
 
 int check_attn(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads, AttnPlan& p) {
@@ -440,11 +461,10 @@ extern "C" int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch
   a.sms = device_sms();
   a.err = device_error_word();
   cudaStream_t st = (cudaStream_t)stream;
-  if (p.prompt) {
-    if (D == 64)
-      return kv->bits == 16 ? launch_prompt<64, 16>(a, p, st) : kv->bits == 8 ? launch_prompt<64, 8>(a, p, st) : launch_prompt<64, 4>(a, p, st);
-    return kv->bits == 16 ? launch_prompt<128, 16>(a, p, st) : kv->bits == 8 ? launch_prompt<128, 8>(a, p, st) : launch_prompt<128, 4>(a, p, st);
-  }
+  if (p.prompt)
+    return on_cache(D, kv->bits, [&](auto d, auto bits) {
+      return launch_prompt<decltype(d)::value, decltype(bits)::value>(a, p, st);
+    });
   return few_rows(D, kv->bits, p.rows, [&](auto d, auto bits, auto nt) {
     return launch_few<decltype(d)::value, decltype(bits)::value, decltype(nt)::value>(a, st);
   });

@@ -203,13 +203,17 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Append.  A warp owns IT * (256 / D) consecutive heads (q heads, then k,
-// then v) of one token: D / 8 lanes per head, eight values per lane, so a
-// head's row moves as one contiguous run, the RMSNorm and the quantizer's
-// min / max are shuffles within the head's lanes, and the token's sequence,
-// page and cos / sin are looked up once per warp.  The rotation's partner
-// values (rot/2 apart) are rot/16 lanes away.  fp32 throughout, rounded
-// once; products and sums of the rotation are rounded separately.
+// Append.  Memory bound: every head is read and written once.  A warp owns a
+// run of one token's heads (q heads, then k, then v), 512 / D at a time.  As in
+// the rotation above a lane holds 16 values of a head, eight pairs of the
+// rotation or 16 neighbours, so that pairs never cross lanes; the RMSNorm and
+// the quantizer's min / max are shuffles within the head's D / 16 lanes, and the
+// token's sequence, page and cos / sin are looked up once per warp.  The loop over
+// the run is not unrolled (unrolled by four, an earlier form outgrew the
+// instruction cache) but loads a step ahead.  The run is as long as leaves the
+// SMs full of warps: long runs share the look-ups, short ones keep a decode
+// step's latency down.  fp32 throughout, rounded once; products and sums of the
+// rotation are rounded separately.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   PagedKv kv;
@@ -223,35 +227,72 @@ struct AppendArgs {
   float eps;
   bf16_t* q_out;
   int64_t ldqo;
+  int run, wpt;          // steps of a warp, warps of a token
   unsigned* err;
 };
 
-template <int D, int IT>
-__global__ void __launch_bounds__(128) paged_append_kernel(AppendArgs a) {
-  constexpr int L = D / 8, HPW = 32 / L;
+// codes rint((x - b) / s), clamped to [0, nb].  A product with 1 / s is within
+// 1e-4 of the quotient (which is below 256), so only quotients that close to a
+// half need the division itself.
+LMX_DEV void quant_codes(const float* x, float s, float b, int nb, uint32_t (&q)[8]) {
+  const float inv = __fdiv_rn(1.0f, s);
+  bool close = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float u = __fmul_rn(__fsub_rn(x[e], b), inv), r = rintf(u);
+    close = close || !(fabsf(__fsub_rn(u, r)) < 0.4998f);
+    q[e] = (uint32_t)(int)fminf(fmaxf(r, 0.0f), (float)nb);
+  }
+  if (close) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      q[e] = (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], b), s)), 0.0f), (float)nb);
+  }
+}
+// eight values' codes to a row
+template <int BITS>
+LMX_DEV void store_codes(uint8_t* dst, const uint32_t (&q)[8]) {
+  if constexpr (BITS == 8) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24),
+                                                q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+  } else {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= q[e] << (4 * e);
+    *reinterpret_cast<uint32_t*>(dst) = w;
+  }
+}
+
+template <int D, int BITS>
+__global__ void __launch_bounds__(128, 7) paged_append_kernel(AppendArgs a) {
+  constexpr int U = D / 16, HPW = 32 / U, NG = D / 64;
   grid_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int nh = a.heads + 2 * a.kv.Hk, wpt = (nh + HPW * IT - 1) / (HPW * IT);
+  const int nh = a.heads + 2 * a.kv.Hk;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (int64_t)a.b.tokens * wpt) return;
-  const int t = (int)(w / wpt), h0 = (int)(w % wpt) * HPW * IT;
-  const int i = lane % L, sub = lane / L;
+  if (w >= (int64_t)a.b.tokens * a.wpt) return;
+  const int t = (int)(w / a.wpt), u = lane % U, sub = lane / U;
+  int h = (int)(w % a.wpt) * a.run * HPW + sub;  // this lane's head; the warp's steps are HPW apart
+  const int end = min(nh, h - sub + a.run * HPW);
+  // this lane's two runs of eight values
+  const bool turns = a.ct && 16 * u < a.rot, halves = turns && !a.inter;
+  const int d0 = halves ? 8 * u : 16 * u, d1 = halves ? a.rot / 2 + 8 * u : d0 + 8;
 
-  // the rows do not depend on the token's place: load them first
-  uint4 raw[IT];
-  float x[8];
-#pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    const int h = h0 + it * HPW + sub;
-    raw[it] = make_uint4(0, 0, 0, 0);
-    if (h < nh) {
-      const bf16_t* src = h < a.heads ? a.q + (int64_t)h * D
-                          : h < a.heads + a.kv.Hk ? a.k + (int64_t)(h - a.heads) * D
-                                                  : a.v + (int64_t)(h - a.heads - a.kv.Hk) * D;
-      raw[it] = *reinterpret_cast<const uint4*>(src + (int64_t)t * a.ld + 8 * i);
+  auto load = [&](int hh, uint4& v0, uint4& v1) {
+    if (hh < end) {
+      const bf16_t* src = hh < a.heads ? a.q + (int64_t)hh * D
+                          : hh < a.heads + a.kv.Hk ? a.k + (int64_t)(hh - a.heads) * D
+                                                   : a.v + (int64_t)(hh - a.heads - a.kv.Hk) * D;
+      const bool v = hh >= a.heads + a.kv.Hk;  // v heads are not turned: any 16 values do
+      src += (int64_t)t * a.ld;
+      v0 = *reinterpret_cast<const uint4*>(src + (v ? 16 * u : d0));
+      v1 = *reinterpret_cast<const uint4*>(src + (v ? 16 * u + 8 : d1));
     }
-  }
+  };
+  // the rows do not depend on the token's place: load the first before looking it up
+  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0;
+  load(h, n0, n1);
   const int seq = paged_seq(a.b, t, lane);
   if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;  // padding
   const int pos = __ldg(a.b.kv_len + seq) - (__ldg(a.b.q_start + seq + 1) - t);
@@ -261,146 +302,139 @@ __global__ void __launch_bounds__(128) paged_append_kernel(AppendArgs a) {
     if (a.ct && pos >= a.positions) row = -1;
     if (row < 0 && lane == 0) atomicExch(a.err, kPagedErr);
   }
-  const int RL = a.ct ? a.rot / 8 : 0;  // rotated lanes of a head
   float c[8], s[8];
-  if (row >= 0 && i < RL) {
-    const int half = a.rot / 2;
-    if (a.inter) {  // four pairs per lane
-      const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.ct + (int64_t)pos * half + 4 * i));
-      const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.st + (int64_t)pos * half + 4 * i));
-      c[0] = c4.x; c[1] = c4.y; c[2] = c4.z; c[3] = c4.w;
-      s[0] = s4.x; s[1] = s4.y; s[2] = s4.z; s[3] = s4.w;
-    } else {
-      const int m = i < RL / 2 ? i : i - RL / 2;
-      load8f(a.ct + (int64_t)pos * half + 8 * m, c);
-      load8f(a.st + (int64_t)pos * half + 8 * m, s);
-    }
+  if (turns && row >= 0) {
+    load8f(a.ct + (int64_t)pos * (a.rot / 2) + 8 * u, c);
+    load8f(a.st + (int64_t)pos * (a.rot / 2) + 8 * u, s);
   }
-  const int partner = i < RL ? (i < RL / 2 ? i + RL / 2 : i - RL / 2) : i;
 
-#pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    const int h = h0 + it * HPW + sub;
-    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv.Hk, live = h < nh;
-    bf8_unpack(raw[it], x);
+#pragma unroll 1
+  for (; h - sub < end; h += HPW) {  // warp-uniform
+    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv.Hk, live = h < end;
+    float x[16];
+    bf8_unpack(n0, *reinterpret_cast<float(*)[8]>(x));
+    bf8_unpack(n1, *reinterpret_cast<float(*)[8]>(x + 8));
+    load(h + HPW, n0, n1);
+    const int e0 = is_q || is_k ? d0 : 16 * u, e1 = is_q || is_k ? d1 : 16 * u + 8;
     if (a.qn) {
       float p = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p = __fmaf_rn(x[e], x[e], p);
-      p = warp_sum_xor(p, L / 2, 1);
+      for (int e = 0; e < 16; ++e) p = __fmaf_rn(x[e], x[e], p);
+      p = warp_sum_xor(p, U / 2, 1);
       if (is_q || is_k) {
-        const float f = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(p, (float)D), a.eps)));
-        float wn[8];
-        bf8_unpack(__ldg(reinterpret_cast<const uint4*>((is_q ? a.qn : a.kn) + 8 * i)), wn);
+        const float f = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fmul_rn(p, 1.0f / D), a.eps)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], f), wn[e]);
+        for (int k = 0; k < 2; ++k) {
+          float wn[8];
+          bf8_unpack(__ldg(reinterpret_cast<const uint4*>((is_q ? a.qn : a.kn) + (k ? e1 : e0))), wn);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[8 * k + e] = __fmul_rn(__fmul_rn(x[8 * k + e], f), wn[e]);
+        }
       }
     }
-    if (RL && !a.inter) {
-      float y[8];
+    if (turns && row >= 0 && (is_q || is_k)) {
+      if (a.inter) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], sub * L + partner);
-      if ((is_q || is_k) && i < RL && row >= 0) {
+        for (int e = 0; e < 8; ++e) {
+          const float xa = x[2 * e], xb = x[2 * e + 1];
+          x[2 * e] = __fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e]));
+          x[2 * e + 1] = __fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e]));
+        }
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[e] = i < RL / 2 ? __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]))
-                            : __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]));
+        for (int e = 0; e < 8; ++e) {
+          const float xa = x[e], xb = x[8 + e];
+          x[e] = __fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e]));
+          x[8 + e] = __fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e]));
+        }
       }
-    } else if ((is_q || is_k) && i < RL && row >= 0) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float xa = x[2 * e], xb = x[2 * e + 1];
-        x[2 * e] = __fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e]));
-        x[2 * e + 1] = __fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e]));
+    }
+    const float(&x0)[8] = *reinterpret_cast<const float(*)[8]>(x), (&x1)[8] = *reinterpret_cast<const float(*)[8]>(x + 8);
+    if (is_q || BITS == 16) {  // bf16 rows: of q_out, or of the cache
+      const int hk = is_k ? h - a.heads : h - a.heads - a.kv.Hk;
+      bf16_t* dst = is_q ? a.q_out + (int64_t)t * a.ldqo + (int64_t)h * D
+                         : reinterpret_cast<bf16_t*>(is_k ? a.kv.k : a.kv.v) + (row + (int64_t)hk * a.kv.P) * D;
+      uint4 o0 = bf8_pack(x0), o1 = bf8_pack(x1);
+      if (row < 0) o0 = o1 = make_uint4(0, 0, 0, 0);
+      if (live && (is_q || row >= 0)) {
+        *reinterpret_cast<uint4*>(dst + e0) = o0;
+        *reinterpret_cast<uint4*>(dst + e1) = o1;
       }
     }
-    if (is_q) {
-      if (row < 0)
+    if constexpr (BITS != 16) {
+      if (h - sub + HPW <= a.heads) continue;  // q heads only
+      // min / max of each group of 64 over the head's lanes
+      float lo[2], hi[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-      *reinterpret_cast<uint4*>(a.q_out + (int64_t)t * a.ldqo + (int64_t)h * D + 8 * i) = bf8_pack(x);
-    }
-    const int hk = is_k ? h - a.heads : h - a.heads - a.kv.Hk;
-    const int64_t r = row + (int64_t)hk * a.kv.P;
-    if (a.kv.bits == 16) {
-      if (!is_q && live && row >= 0)
-        *reinterpret_cast<uint4*>((is_k ? a.kv.k : a.kv.v) + (r * D + 8 * i) * 2) = bf8_pack(x);
-      continue;
-    }
-    // min / max of a group of 64 = 8 lanes
-    float mn = x[0], mx = x[0];
+      for (int k = 0; k < 2; ++k) {
+        lo[k] = hi[k] = x[8 * k];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) { mn = fminf(mn, x[e]); mx = fmaxf(mx, x[e]); }
+        for (int e = 1; e < 8; ++e) {
+          lo[k] = fminf(lo[k], x[8 * k + e]);
+          hi[k] = fmaxf(hi[k], x[8 * k + e]);
+        }
+      }
+      constexpr int nb = (1 << BITS) - 1;
+      bf16_t sb[NG], bb[NG];
 #pragma unroll
-    for (int off = 4; off >= 1; off >>= 1) {
-      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    }
-    if (is_q || !live || row < 0) continue;
-    const int nb = (1 << a.kv.bits) - 1;
-    bf16_t sb = f2bf(__fdiv_rn(__fsub_rn(mx, mn), (float)nb));
-    if (bf2f(sb) == 0.0f) sb = f2bf(1.0f);
-    const bf16_t bb = f2bf(mn);
-    const float sc = bf2f(sb), bi = bf2f(bb);
-    uint32_t q[8];
+      for (int g = 0; g < NG; ++g) {
+        float mn = INFINITY, mx = -INFINITY;
+        if (e0 / 64 == g) { mn = lo[0]; mx = hi[0]; }
+        if (e1 / 64 == g) { mn = fminf(mn, lo[1]); mx = fmaxf(mx, hi[1]); }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int v = (int)rintf(__fdiv_rn(__fsub_rn(x[e], bi), sc));
-      q[e] = (uint32_t)(v < 0 ? 0 : (v > nb ? nb : v));
-    }
-    uint8_t* dst = is_k ? a.kv.k : a.kv.v;
-    if (a.kv.bits == 8) {
-      *reinterpret_cast<uint2*>(dst + r * D + 8 * i) =
-          make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
-    } else {
-      uint32_t wd = 0;
+        for (int off = U / 2; off >= 1; off >>= 1) {
+          mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        }
+        sb[g] = f2bf(__fdiv_rn(__fsub_rn(mx, mn), (float)nb));
+        if (bf2f(sb[g]) == 0.0f) sb[g] = f2bf(1.0f);
+        bb[g] = f2bf(mn);
+      }
+      if (is_q || !live || row < 0) continue;
+      const int64_t r = row + (int64_t)(is_k ? h - a.heads : h - a.heads - a.kv.Hk) * a.kv.P;
+      uint8_t* dst = (is_k ? a.kv.k : a.kv.v) + r * (D * BITS / 8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) wd |= q[e] << (4 * e);
-      *reinterpret_cast<uint32_t*>(dst + r * (D / 2) + 4 * i) = wd;
-    }
-    if ((i & 7) == 0) {
-      (is_k ? a.kv.ks : a.kv.vs)[r * (D / 64) + (i >> 3)] = sb;
-      (is_k ? a.kv.kb : a.kv.vb)[r * (D / 64) + (i >> 3)] = bb;
+      for (int k = 0; k < 2; ++k) {
+        const int d = k ? e1 : e0, g = NG == 2 ? d / 64 : 0;
+        const float sc = bf2f(NG == 2 && g ? sb[NG - 1] : sb[0]), bi = bf2f(NG == 2 && g ? bb[NG - 1] : bb[0]);
+        uint32_t q[8];
+        quant_codes(x + 8 * k, sc, bi, nb, q);
+        store_codes<BITS>(dst + d * BITS / 8, q);
+      }
+      if (u == 0) {
+        bf16_t *ps = (is_k ? a.kv.ks : a.kv.vs) + r * NG, *pb = (is_k ? a.kv.kb : a.kv.vb) + r * NG;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          ps[g] = sb[g];
+          pb[g] = bb[g];
+        }
+      }
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Gather: the batch's rows back as bf16(fma(scale, code, bias)).  A warp owns
-// one token, its lanes the 8-value chunks of the K heads, then the V heads.
+// Gather: the batch's rows back as bf16(fma(scale, code, bias)).  A lane owns
+// one 8-value chunk of a token's K heads, then V heads, at a time; a warp `run`
+// times 32 chunks of one token.
 // ---------------------------------------------------------------------------
 struct GatherArgs {
   PagedKv kv;
   PagedBatch b;
   bf16_t *k, *v;
+  int run, wpt;  // steps of a warp, warps of a token
   unsigned* err;
 };
 
-// eight codes of a row -> values
-LMX_DEV uint4 paged_dequant8(int bits, const uint8_t* base, const bf16_t* sc, const bf16_t* bi, int64_t r, int D, int c) {
-  const float s = bf2f(__ldg(sc + r * (D / 64) + c / 8)), b = bf2f(__ldg(bi + r * (D / 64) + c / 8));
-  float x[8];
-  if (bits == 8) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(base + r * D + 8 * c));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(s, (float)(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu), b);
-  } else {
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(base + r * (D / 2) + 4 * c));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(s, (float)((w >> (4 * e)) & 0xfu), b);
-  }
-  return bf8_pack(x);
-}
-
-template <int D>
+template <int D, int BITS>
 __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
   constexpr int L = D / 8;
   grid_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= a.b.tokens) return;
-  const int t = (int)w;
+  if (w >= (int64_t)a.b.tokens * a.wpt) return;
+  const int t = (int)(w / a.wpt);
   const int seq = paged_seq(a.b, t, lane);
   if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;  // padding
   const int pos = __ldg(a.b.kv_len + seq) - (__ldg(a.b.q_start + seq + 1) - t);
@@ -409,9 +443,9 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
     row = paged_row(a.kv, a.b, seq, pos);
     if (row < 0 && lane == 0) atomicExch(a.err, kPagedErr);
   }
-  const int n = a.kv.Hk * L;
-#pragma unroll 4
-  for (int c = lane; c < 2 * n; c += 32) {
+  const int n = a.kv.Hk * L, c0 = (int)(w % a.wpt) * a.run * 32;
+#pragma unroll 2
+  for (int c = c0 + lane; c < min(2 * n, c0 + a.run * 32); c += 32) {
     const bool is_k = c < n;
     const int at = is_k ? c : c - n, h = at / L, i = at % L;
     bf16_t* dst = is_k ? a.k : a.v;
@@ -420,8 +454,23 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
     if (row >= 0) {
       const int64_t r = row + (int64_t)h * a.kv.P;
       const uint8_t* src = is_k ? a.kv.k : a.kv.v;
-      o = a.kv.bits == 16 ? __ldg(reinterpret_cast<const uint4*>(src + (r * D + 8 * i) * 2))
-                          : paged_dequant8(a.kv.bits, src, is_k ? a.kv.ks : a.kv.vs, is_k ? a.kv.kb : a.kv.vb, r, D, i);
+      if constexpr (BITS == 16) {
+        o = __ldg(reinterpret_cast<const uint4*>(src + (r * D + 8 * i) * 2));
+      } else {
+        const int64_t g = r * (D / 64) + i / 8;
+        const float sc = bf2f(__ldg((is_k ? a.kv.ks : a.kv.vs) + g)), bi = bf2f(__ldg((is_k ? a.kv.kb : a.kv.vb) + g));
+        float x[8];
+        if constexpr (BITS == 8) {
+          const uint2 q = __ldg(reinterpret_cast<const uint2*>(src + r * D + 8 * i));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(sc, (float)(((e < 4 ? q.x : q.y) >> (8 * (e & 3))) & 0xffu), bi);
+        } else {
+          const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(src + r * (D / 2) + 4 * i));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(sc, (float)((q >> (4 * e)) & 0xfu), bi);
+        }
+        o = bf8_pack(x);
+      }
     }
     *reinterpret_cast<uint4*>(dst + (int64_t)t * n * 8 + 8 * at) = o;
   }

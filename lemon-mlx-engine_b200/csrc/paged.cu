@@ -100,15 +100,14 @@ auto on_cache(int D, int bits, F f) {
   return D == 64 ? on_bits(std::integral_constant<int, 64>()) : on_bits(std::integral_constant<int, 128>());
 }
 
+
 // A token's `steps` split over wpt warps of `run` steps: one warp a step while
-// that is at most RUNW warps per SM, longer runs beyond.
-#ifndef RUNW
-#define RUNW 64
-#endif
+// that is at most 64 warps per SM, longer runs beyond (16 to 128 measure alike).
 void warp_runs(int tokens, int steps, int& run, int& wpt) {
-  const int64_t warps = (int64_t)device_sms() * RUNW;
+  const int64_t warps = (int64_t)device_sms() * 64;
   run = (int)std::min<int64_t>(steps, std::max<int64_t>(1, (int64_t)tokens * steps / warps));
   wpt = (steps + run - 1) / run;
+  run = (steps + wpt - 1) / wpt;
 }
 
 int grid_of(int64_t blocks, unsigned& grid, const char* who) {
@@ -251,7 +250,7 @@ extern "C" int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* b
     return set_error(LMX_ERR_INVALID, "paged_gather: k_out and v_out must be 16-byte aligned");
   if (batch->tokens == 0 || batch->seqs == 0 || (!k_out && !v_out)) return LMX_OK;
   GatherArgs a{dev_kv(*kv), dev_batch(*batch), (bf16_t*)k_out, (bf16_t*)v_out, 0, 0, device_error_word()};
-  warp_runs(batch->tokens, (2 * kv->kv_heads * kv->head_dim / 8 + 31) / 32, a.run, a.wpt);
+  warp_runs(batch->tokens, (2 * kv->kv_heads * kv->head_dim / 16 + 31) / 32, a.run, a.wpt);
   unsigned grid;
   if ((rc = grid_of(((int64_t)batch->tokens * a.wpt + 3) / 4, grid, "paged_gather"))) return rc;
   return cuda_check(on_cache(kv->head_dim, kv->bits, [&](auto d, auto bits) {

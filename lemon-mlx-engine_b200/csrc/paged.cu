@@ -386,10 +386,8 @@ int launch_prompt(const PagedAttnArgs& a, const AttnPlan& pl, cudaStream_t st) {
     if (rc) return rc;
     attr_set[d & 63] = true;
   }
-  rc = cuda_check(lmx_launch(paged_prompt_plan_kernel, dim3(1), dim3(1024), 0, st, true, p), "paged_attention: plan launch");
-  if (!rc)
-    rc = cuda_check(lmx_launch(paged_prompt_kernel<D, BITS>, dim3(a.nctas), dim3(prompt_threads(BITS)), smem, st, true, mp, p),
-                    "paged_attention: prompt launch");
+  rc = cuda_check(lmx_launch(paged_prompt_kernel<D, BITS>, dim3(a.nctas), dim3(prompt_threads(BITS)), smem, st, true, mp, p),
+                  "paged_attention: prompt launch");
   if (!rc)
     rc = cuda_check(lmx_launch(paged_prompt_join_kernel<D>, dim3(a.nctas, kPromptRows / 32), dim3(128), 0, st, true, p),
                     "paged_attention: join launch");

@@ -30,7 +30,7 @@
 // laid end to end, each item with a fixed cost of its own in front, and divided
 // evenly over one CTA per SM; items that cross a
 // boundary leave fp32 partials that paged_prompt_join_kernel adds in order.
-// The division is computed once, by paged_prompt_plan_kernel.
+// Every CTA works the division out for itself (prompt_plan).
 #pragma once
 #include "paged.cuh"
 #include "sm100.cuh"
@@ -38,9 +38,10 @@
 namespace lmx {
 
 static constexpr int kPromptSoftmaxWarps = 16;  // per row tile: two halves of four
-// + MMA, loads, V clearing (idle for quantized caches) and one spare; + four
+static constexpr int kPromptDeqWarps = 8;
+// + MMA, loads, V clearing (idle for quantized caches) and one spare; + the
 // warps that dequantize
-constexpr int prompt_threads(int bits) { return 32 * kPromptSoftmaxWarps + (bits == 16 ? 128 : 256); }
+constexpr int prompt_threads(int bits) { return 32 * (kPromptSoftmaxWarps + 4 + (bits == 16 ? 0 : kPromptDeqWarps)); }
 static constexpr int kPromptRows = 256;  // rows of a pair
 
 struct PromptArgs {
@@ -79,18 +80,20 @@ LMX_DEV void prompt_pair(const PromptArgs& p, int pair, PromptItem& z) {
   z.nblk = max(1, ((z.hi + 127) >> 7) - z.kb);
 }
 
-// Blocks before each sequence, and where each CTA begins.
-__global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
-  __shared__ int64_t pre[kPagedMaxSeqs + 1];
-  __shared__ int64_t wsum[32];
-  grid_wait();
-  grid_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// Where a CTA begins, and how much it has.
+struct PromptShare {
+  int4 start;    // as PromptArgs::start
+  int64_t left;  // blocks and item costs
+};
+// The division, by a whole CTA for itself, into shared memory (and start[] for
+// the join); `pre` (seqs + 1) gets the blocks before each sequence.
+LMX_DEV void prompt_plan(const PromptArgs& p, int64_t* pre, int64_t* wsum, PromptShare* share) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int seqs = p.a.b.seqs;
-  for (int s = warp; s < seqs; s += 32) {
+  for (int s = warp; s < seqs; s += warps) {
     PromptItem z;
     prompt_seq(p, s, z);
-    if (lane == 0 && z.nnew > 0 && z.kvlen > z.len) atomicExch(p.a.err, kPagedErr);
+    if (blockIdx.x == 0 && lane == 0 && z.nnew > 0 && z.kvlen > z.len) atomicExch(p.a.err, kPagedErr);
     int64_t n = 0;
     for (int i = lane; i < z.pairs; i += 32) {
       prompt_pair(p, i, z);
@@ -102,10 +105,11 @@ __global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
   }
   if (tid == 0) pre[0] = 0;
   __syncthreads();
-  // inclusive scan, two entries per thread
-  const int i0 = 2 * tid + 1, i1 = i0 + 1;
-  const int64_t v0 = i0 <= seqs ? pre[i0] : 0, v1 = i1 <= seqs ? pre[i1] : 0;
-  int64_t v = v0 + v1;
+  // inclusive scan, `per` consecutive entries a thread
+  const int per = (seqs + blockDim.x - 1) / blockDim.x, i0 = tid * per + 1;
+  int64_t v = 0;
+  for (int i = i0; i < i0 + per && i <= seqs; ++i) v += pre[i];
+  const int64_t own = v;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const int64_t o = __shfl_up_sync(0xffffffffu, v, off);
@@ -114,14 +118,15 @@ __global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
   if (lane == 31) wsum[warp] = v;
   __syncthreads();
   for (int w = 0; w < warp; ++w) v += wsum[w];
-  if (i0 <= seqs) pre[i0] = v - v1;
-  if (i1 <= seqs) pre[i1] = v;
+  v -= own;
+  for (int i = i0; i < i0 + per && i <= seqs; ++i) pre[i] = v += pre[i];
   __syncthreads();
-  const int64_t total = pre[seqs];
-  if (tid == 0) p.a.prefix[0] = total;
-  const int n = (int)(total < p.a.nctas ? total : p.a.nctas);
-  for (int c = warp; c < n; c += 32) {
-    const int64_t at = total * c / n;
+  const int64_t total = pre[seqs], n = total < p.a.nctas ? total : p.a.nctas;
+  if (blockIdx.x == 0 && tid == 0) p.a.prefix[0] = total;
+  if (tid == 0) share->left = 0;
+  if (warp == 0 && blockIdx.x < n) {
+    const int64_t at = paged_share(total, blockIdx.x, n);
+    if (lane == 0) share->left = paged_share(total, blockIdx.x + 1, n) - at;
     int s = 0, e = seqs;
     while (e - s > 1) {
       const int mid = (s + e) / 2;
@@ -131,9 +136,9 @@ __global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
     while (pre[s + 1] <= at) ++s;
     PromptItem z;
     prompt_seq(p, s, z);
-    const int64_t per = (pre[s + 1] - pre[s]) / p.a.kv.Hk, loc = at - pre[s];
-    const int h = (int)(loc / per);
-    int rem = (int)(loc % per);
+    const int64_t of_head = (pre[s + 1] - pre[s]) / p.a.kv.Hk, loc = at - pre[s];
+    const int h = (int)(loc / of_head);
+    int64_t rem = loc - h * of_head;
     for (int base = 0;; base += 32) {  // the pair that holds block rem of this head
       int nb = 0;
       if (base + lane < z.pairs) {
@@ -150,12 +155,15 @@ __global__ void __launch_bounds__(1024) paged_prompt_plan_kernel(PromptArgs p) {
       if (past) {
         const int l = __ffs(past) - 1;
         const int before = __shfl_sync(0xffffffffu, inc - nb, l);
-        if (lane == 0) p.start[c] = make_int4(s, h, base + l, rem - before);
+        if (lane == 0) p.start[blockIdx.x] = share->start = make_int4(s, h, base + l, (int)rem - before);
         break;
       }
       rem -= __shfl_sync(0xffffffffu, inc, 31);
     }
   }
+  // `pre` lies where the copies land: order these accesses before them
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
 }
 
 // A CTA's walk over its share: one segment (item, blocks [b0, b1)) at a time.
@@ -173,12 +181,10 @@ struct PromptWalk {
     b0 = max(0, off - p.cost);
     b1 = max(0, off + len - p.cost);
   }
-  LMX_DEV void begin(const PromptArgs& p) {
-    const int64_t total = p.a.prefix[0], n = total < p.a.nctas ? total : p.a.nctas;
-    left = 0;
-    if (blockIdx.x >= n) return;
-    left = total * (blockIdx.x + 1) / n - total * blockIdx.x / n;
-    const int4 s = p.start[blockIdx.x];
+  LMX_DEV void begin(const PromptArgs& p, const PromptShare* share) {
+    left = share->left;
+    if (left <= 0) return;
+    const int4 s = share->start;
     seq = s.x; h = s.y; pair = s.z;
     prompt_seq(p, seq, z);
     prompt_pair(p, pair, z);
@@ -406,8 +412,8 @@ struct PromptSmem {
   // overlapped.  Without it the CTAs that get a prompt's short first items take
   // 27% longer than the others (8192 tokens, 64 heads); swept 0 to 4 blocks.
   static constexpr int COST = D == 128 ? 4 : 2;
-  static constexpr int BARS = (12 + 2 * NS + 2 * NR + 1) * 8 + 8;
-  static constexpr int XCH = (BARS + 127) / 128 * 128;
+  static constexpr int BARS = ((12 + 2 * NS + 1 + 2 * NR) * 8 + 15) / 16 * 16;
+  static constexpr int XCH = (BARS + 48 + 127) / 128 * 128;  // + share, tensor memory's address
   static constexpr int BYTES = 2 * TILE + NS * TILE + NR * RAW + XCH + 2048;  // tiles, barriers, exchange
 };
 
@@ -503,12 +509,13 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
   uint64_t *q_full = bars, *q_free = bars + 1, *vfix = bars + 2, *s_full = bars + 3, *p_ready = bars + 5,
            *o_full = bars + 7, *o_free = bars + 9, *drain = bars + 11, *kv_full = bars + 12, *kv_free = kv_full + NS;
   uint64_t *q_raw = kv_free + NS, *raw_full = q_raw + 1, *raw_free = raw_full + SM::NR;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_free + SM::NR);
+  PromptShare* share = reinterpret_cast<PromptShare*>(rest + SM::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share + 1);
   float* xch = reinterpret_cast<float*>(rest + SM::XCH);  // [tile][half][128]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, BITS == 16 ? 1 : 4);
+    mbar_init(q_full, BITS == 16 ? 1 : kPromptDeqWarps);
     mbar_init(q_raw, 1);
     mbar_init(q_free, 1);
     mbar_init(vfix, 1);
@@ -520,12 +527,12 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       mbar_init(o_free + i, 8);
     }
     for (int i = 0; i < NS; ++i) {
-      mbar_init(kv_full + i, BITS == 16 ? 1 : 4);
+      mbar_init(kv_full + i, BITS == 16 ? 1 : kPromptDeqWarps);
       mbar_init(kv_free + i, BITS == 16 ? 2 : 1);  // the MMAs' commit and the warp that clears V
     }
     for (int i = 0; i < SM::NR; ++i) {
       mbar_init(raw_full + i, 1);
-      mbar_init(raw_free + i, 4);
+      mbar_init(raw_free + i, kPromptDeqWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -540,6 +547,8 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
   const uint32_t tmem = *tmem_slot;
   grid_wait();
   grid_launch_dependents();
+  // the tiles' memory is free until the first load
+  prompt_plan(p, reinterpret_cast<int64_t*>(KV), reinterpret_cast<int64_t*>(xch), share);
   unsigned* err = p.a.err;
   PromptWalk w;
 
@@ -560,7 +569,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
     bool ok = true;
     // A wait that gives up is the last one; the rest then runs through on
     // whatever is there, because the halves' barriers need all warps.
-    for (w.begin(p); w.live(); w.next(p)) {
+    for (w.begin(p, share); w.live(); w.next(p)) {
       if (tile == 1 && !w.second(p)) continue;
       const int t = r / G, tok = w.z.t0 + tile * p.TT + t;  // token of the sequence
       const bool row = t < p.TT && tok < w.z.nnew;
@@ -667,52 +676,45 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
     }
   } else if (BITS != 16 && warp >= kMma + 4) {
     // ----------------------------- dequantize -----------------------------
-    // A lane turns 16 codes of a row at a time; a warp owns 32 rows of each
+    // A lane turns 16 codes of a row at a time; a warp owns 16 rows of each
     // tile.  The scales of the next tile of the same kind are loaded before
     // this one is converted.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if constexpr (BITS != 16) {
-      constexpr int U = D / 16, RPI = 32 / U, IT = 32 / RPI, NG = D / 64;  // units per row, rows per pass, passes
-      const int dw = warp - kMma - 4, u = lane % U, r0 = dw * 32 + lane / U;
+      constexpr int U = D / 16, RPI = 32 / U, IT = 16 / RPI, NG = D / 64;  // units per row, rows per pass, passes
+      const int dw = warp - kMma - 4, u = lane % U, r0 = dw * 16 + lane / U;
       const PagedKv& kv = p.a.kv;
       int st = 0, rs = 0;
       uint32_t pst = 1, prs = 0, pq = 0;  // parities of kv_free, raw_full, q_raw
       bool ok = true;
-      // rows of the head: the warp's first and second 16 keys of block b (-1: none)
-      auto rows_of = [&](int b, int64_t (&at)[2]) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int key = ((w.z.kb + b) << 7) + dw * 32 + 16 * k;
-          at[k] = -1;
-          if (b < w.b1 && key < w.z.hi && key + 16 > w.z.lo) {
-            const int64_t r = paged_row(kv, p.a.b, w.seq, key);
-            at[k] = r < 0 ? -1 : r + (int64_t)w.h * kv.P;
-          }
-        }
+      // row of the head for the warp's 16 keys of block b (-1: none)
+      auto row_of = [&](int b) -> int64_t {
+        const int key = ((w.z.kb + b) << 7) + dw * 16;
+        if (b >= w.b1 || key >= w.z.hi || key + 16 <= w.z.lo) return -1;
+        const int64_t r = paged_row(kv, p.a.b, w.seq, key);
+        return r < 0 ? -1 : r + (int64_t)w.h * kv.P;
       };
-      auto load_sb = [&](const bf16_t* sc, const bf16_t* bi, int b, const int64_t (&at)[2], uint32_t (&sb)[IT]) {
+      auto load_sb = [&](const bf16_t* sc, const bf16_t* bi, int b, int64_t at, uint32_t (&sb)[IT]) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-          const int r = lane / U + RPI * i;  // of the warp's 32
+          const int r = lane / U + RPI * i;  // of the warp's 16
           sb[i] = 0;                         // rows that are not there read as zeros
-          const int64_t base = at[(RPI * i) >> 4];
-          if (base >= 0 && ((w.z.kb + b) << 7) + dw * 32 + r < w.z.len) {
-            const int64_t x = (base + (r & 15)) * NG + u / (U / NG);
+          if (at >= 0 && ((w.z.kb + b) << 7) + dw * 16 + r < w.z.len) {
+            const int64_t x = (at + r) * NG + u / (U / NG);
             sb[i] = (uint32_t)__ldg(sc + x) | ((uint32_t)__ldg(bi + x) << 16);
           }
         }
       };
-      for (w.begin(p); ok && w.live(); w.next(p)) {
-        int64_t at[2];
+      for (w.begin(p, share); ok && w.live(); w.next(p)) {
         uint32_t sk[IT], sv[IT];
-        rows_of(w.b0, at);
+        int64_t at = row_of(w.b0);
         load_sb(kv.ks, kv.kb, w.b0, at, sk);
         load_sb(kv.vs, kv.vb, w.b0, at, sv);
         ok = prompt_warp_wait(q_raw, pq, err, 0x53u);
         if (!ok) break;
         pq ^= 1;
         const int tiles = w.second(p) ? 2 : 1;
-        for (int i = threadIdx.x & 127; i < tiles * (TILE / 16); i += 128) {
+        for (int i = dw * 32 + lane; i < tiles * (TILE / 16); i += 32 * kPromptDeqWarps) {
           uint4* q = reinterpret_cast<uint4*>(Qs) + i;
           *q = prompt_q8<BITS>(*q);
         }
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
         for (int b = w.b0; b < w.b1 && ok; ++b) {
-          rows_of(b + 1, at);
+          at = row_of(b + 1);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t(&sb)[IT] = h ? sv : sk;
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
         ok = ok && prompt_warp_wait(bar, parity, err, code);
         return ok;
       };
-      for (w.begin(p); ok && w.live(); w.next(p)) {
+      for (w.begin(p, share); ok && w.live(); w.next(p)) {
         const int tiles = w.second(p) ? 2 : 1, n = w.b1 - w.b0;
         if (!wait(q_full, pq, 0x47u) || !wait(kv_full + st, pst, 0x48u)) break;
         pq ^= 1;
@@ -857,7 +859,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       uint32_t pst = 1, pq = 1;
       int issued = 0;
       bool ok = true, started = false;
-      for (w.begin(p); ok && w.live(); w.next(p)) {
+      for (w.begin(p, share); ok && w.live(); w.next(p)) {
         const int tiles = w.second(p) ? 2 : 1;
         ok = prompt_warp_wait(q_free, pq, err, 0x4Cu);
         if (!ok) break;
@@ -903,7 +905,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       int st = 0;
       uint32_t pst = 0;
       bool ok = true;
-      for (w.begin(p); ok && w.live(); w.next(p)) {
+      for (w.begin(p, share); ok && w.live(); w.next(p)) {
         for (int b = w.b0; b < w.b1 && ok; ++b) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
@@ -948,16 +950,17 @@ __global__ void __launch_bounds__(128) paged_prompt_join_kernel(const __grid_con
   if (c >= n || c == 0) return;
   const int4 s = p.start[c];
   if (s.w <= p.cost) return;               // begins with its item
-  const int64_t i0 = total * c / n - s.w;           // where the item begins
-  if (total * (c - 1) / n - i0 > p.cost) return;  // CTA c - 1 begins inside it too
+  const int64_t i0 = paged_share(total, c, n) - s.w;  // where the item begins
+  const int64_t before = paged_share(total, c - 1, n);
+  if (before - i0 > p.cost) return;  // CTA c - 1 begins inside it too
   PromptItem z;
   prompt_seq(p, s.x, z);
   prompt_pair(p, s.z, z);
-  const int64_t c1 = ((i0 + p.cost + z.nblk) * n - 1) / total;  // CTA of its last block
+  const int64_t c1 = paged_owner(total, i0 + p.cost + z.nblk - 1, n);  // CTA of its last block
   const int row = blockIdx.y * 32 + (threadIdx.x & 31), tile = row >> 7, r = row & 127;
   const int t = r / p.a.G, tok = z.t0 + tile * p.TT + t;
   if (t >= p.TT || tok >= z.nnew) return;
-  const int64_t slot0 = 2 * (c - 1) + (total * (c - 1) / n < i0 ? 1 : 0);
+  const int64_t slot0 = 2 * (c - 1) + (before < i0 ? 1 : 0);
   auto slot_of = [&](int64_t k) { return k == c - 1 ? slot0 : 2 * k; };
   float M = -INFINITY;
   for (int64_t k = c - 1; k <= c1; ++k) M = fmaxf(M, p.a.ml[(slot_of(k) * kPromptRows + row) * 2]);

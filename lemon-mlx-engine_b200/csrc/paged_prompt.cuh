@@ -679,7 +679,12 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
     // A lane turns 16 codes of a row at a time; a warp owns 16 rows of each
     // tile.  The scales of the next tile of the same kind are loaded before
     // this one is converted.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    // registers per thread at launch 72 (65,536 over 896 threads): the splits of
+    // 504 = 7 * 72 are 4 x 88 + 56 + 2 x 48, and for 4 bits, whose unpacking holds
+    // more at once, 4 x 88 + 40 + 2 x 56 (2048-token prompt of 64 heads 144 -> 136 us;
+    // 8 bits 122 -> 128)
+    if constexpr (BITS == 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if constexpr (BITS != 16) {
       constexpr int U = D / 16, RPI = 32 / U, IT = 16 / RPI, NG = D / 64;  // units per row, rows per pass, passes
       const int dw = warp - kMma - 4, u = lane % U, r0 = dw * 16 + lane / U;
@@ -758,7 +763,8 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
     }
   } else {
     if constexpr (BITS == 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else if constexpr (BITS == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == kMma) {
       // ------------------------------ MMA issue ------------------------------
       // A and B bf16 (fp16 for quantized caches: formats 0), D fp32; M = 128

@@ -362,6 +362,7 @@ int launch_prompt(const PagedAttnArgs& a, const AttnPlan& pl, cudaStream_t st) {
   PromptArgs p;
   p.a = a;
   p.TT = 128 / a.G;
+  p.wide = !((uintptr_t)a.out & 31) && a.ldo % 16 == 0;
   p.cost = PromptSmem<D, BITS>::COST;
   p.start = (int4*)((uint8_t*)a.prefix + pl.start);
   PromptMaps mp;

@@ -47,6 +47,7 @@ static constexpr int kPromptRows = 256;  // rows of a pair
 struct PromptArgs {
   PagedAttnArgs a;   // nctas = CTAs of the grid; prefix[0] = total blocks; ml / part per slot of 256 rows
   int TT;            // tokens of one row tile
+  int wide;          // output rows are 32-byte aligned
   int cost;          // what an item costs beside its blocks, in blocks (PromptSmem)
   int4* start;       // [nctas] where a CTA begins: sequence, head, pair, offset into the item
 };
@@ -410,8 +411,10 @@ struct PromptSmem {
   static constexpr int NS = D == 128 ? (BITS == 16 ? 5 : 4) : 8;   // K / V stages
   // An item's own cost: its first scores and its last P V and output are not
   // overlapped.  Without it the CTAs that get a prompt's short first items take
-  // 27% longer than the others (8192 tokens, 64 heads); swept 0 to 4 blocks.
-  static constexpr int COST = D == 128 ? 4 : 2;
+  // 27% longer than the others (8192 tokens, 64 heads).  Swept 2 to 5 (128; 2048
+  // tokens of 64 heads 94, 93, 95, 96 us) and 1 to 4 (64; ragged prompts 211,
+  // 203, 210, 217 us).
+  static constexpr int COST = D == 128 ? 3 : 2;
   static constexpr int BARS = ((12 + 2 * NS + 1 + 2 * NR) * 8 + 15) / 16 * 16;
   static constexpr int XCH = (BARS + 48 + 127) / 128 * 128;  // + share, tensor memory's address
   static constexpr int BYTES = 2 * TILE + NS * TILE + NR * RAW + XCH + 2048;  // tiles, barriers, exchange
@@ -486,6 +489,22 @@ LMX_DEV void prompt_order(float (&y)[16]) {
         y[k + i + 4] = t[2 * i + 1];
       }
     }
+  }
+}
+
+// 16 output values; wide: 32-byte aligned, one store (a lane's row is its own, so
+// each store is 32 separate pieces: the fewer the better)
+LMX_DEV void prompt_store16(bf16_t* dst, const float (&o)[16], float f, bool wide) {
+  uint32_t w[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) w[k] = pk_bf2(o[2 * k] * f, o[2 * k + 1] * f);
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
@@ -645,13 +664,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
           tmem_ld16(tO + i, o);
           prompt_order<BITS>(o);
           if (row)
-#pragma unroll
-            for (int k = 0; k < 16; k += 8) {
-              float y[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = o[k + e] * inv;
-              *reinterpret_cast<uint4*>(op + i + k) = bf8_pack(y);
-            }
+            prompt_store16(op + i, o, inv, p.wide);
         }
         if (half == 0 && row && p.a.lse)
           p.a.lse[(int64_t)(w.z.first + tok) * p.a.heads + head] =
@@ -715,17 +728,6 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
         int64_t at = row_of(w.b0);
         load_sb(kv.ks, kv.kb, w.b0, at, sk);
         load_sb(kv.vs, kv.vb, w.b0, at, sv);
-        ok = prompt_warp_wait(q_raw, pq, err, 0x53u);
-        if (!ok) break;
-        pq ^= 1;
-        const int tiles = w.second(p) ? 2 : 1;
-        for (int i = dw * 32 + lane; i < tiles * (TILE / 16); i += 32 * kPromptDeqWarps) {
-          uint4* q = reinterpret_cast<uint4*>(Qs) + i;
-          *q = prompt_q8<BITS>(*q);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
         for (int b = w.b0; b < w.b1 && ok; ++b) {
           at = row_of(b + 1);
 #pragma unroll
@@ -754,6 +756,19 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
             if (lane == 0) {
               mbar_arrive(kv_full + st);
               mbar_arrive(raw_free + rs);
+            }
+            if (h == 0 && b == w.b0) {  // Q comes behind the first tiles
+              ok = prompt_warp_wait(q_raw, pq, err, 0x53u);
+              if (!ok) break;
+              pq ^= 1;
+              const int chunks = (w.second(p) ? 2 : 1) * (TILE / 16);
+              for (int k = dw * 32 + lane; k < chunks; k += 32 * kPromptDeqWarps) {
+                uint4* q = reinterpret_cast<uint4*>(Qs) + k;
+                *q = prompt_q8<BITS>(*q);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(q_full);
             }
             if (++st == NS) { st = 0; pst ^= 1; }
             if (++rs == SM::NR) { rs = 0; prs ^= 1; }
@@ -867,16 +882,6 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       bool ok = true, started = false;
       for (w.begin(p, share); ok && w.live(); w.next(p)) {
         const int tiles = w.second(p) ? 2 : 1;
-        ok = prompt_warp_wait(q_free, pq, err, 0x4Cu);
-        if (!ok) break;
-        pq ^= 1;
-        started = true;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(qbar, (uint32_t)(tiles * qbytes));
-          for (int i = 0; i < tiles; ++i)
-            for (int h = 0; h < NH; ++h)
-              tma_load_3d(Qs + i * TILE + h * 16384, &mp.q, h * 64, w.h * p.a.G, w.z.first + w.z.t0 + i * p.TT, qbar);
-        }
         for (int b = w.b0; b < w.b1 && ok; ++b) {
           const int key = (w.z.kb + b) * 128 + lane * rows;
           int page = p.a.kv.pages;  // out of range: the box reads as zeros
@@ -899,6 +904,21 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
                             kv ? &mp.v : &mp.k, h * 64, key & (P - 1), w.h, page, full + st);
             ++issued;
             if (++st == N) { st = 0; pst ^= 1; }
+          }
+          if (b == w.b0 && ok) {
+            // Q behind the item's first K and V: its memory is free only when the
+            // previous item's last scores are done
+            ok = prompt_warp_wait(q_free, pq, err, 0x4Cu);
+            if (!ok) break;
+            pq ^= 1;
+            started = true;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(qbar, (uint32_t)(tiles * qbytes));
+              for (int i = 0; i < tiles; ++i)
+                for (int h = 0; h < NH; ++h)
+                  tma_load_3d(Qs + i * TILE + h * 16384, &mp.q, h * 64, w.h * p.a.G, w.z.first + w.z.t0 + i * p.TT, qbar);
+            }
+            __syncwarp();
           }
         }
       }

@@ -338,7 +338,9 @@ int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* batch, void*
  * must hold finite values.  scratch: lmx_paged_attention_scratch_bytes of the
  * same kv / batch / heads (0 and a message in lmx_last_error when the
  * arguments are refused), 16-byte aligned, contents arbitrary; calls that
- * overlap need scratch of their own. */
+ * overlap need scratch of their own.  Waits inside the prompt kernel are
+ * bounded: one that gives up sets the device error word to 0x85 .. 0x95 and
+ * the results are not valid. */
 size_t lmx_paged_attention_scratch_bytes(const lmx_paged_kv* kv, const lmx_paged_batch* batch, int heads);
 int lmx_paged_attention(const lmx_paged_kv* kv, const lmx_paged_batch* batch, const void* q, int64_t ldq, int heads,
                         float scale, int window, void* scratch, size_t scratch_bytes, void* out, int64_t ldo,

@@ -103,9 +103,9 @@ auto on_cache(int D, int bits, F f) {
 
 // A token's `steps` split over wpt warps of `run` steps: one warp a step while
 // that is at most 64 warps per SM, longer runs beyond (16 to 128 measure alike).
-void warp_runs(int tokens, int steps, int& run, int& wpt) {
+void warp_runs(int tokens, int steps, int most, int& run, int& wpt) {
   const int64_t warps = (int64_t)device_sms() * 64;
-  run = (int)std::min<int64_t>(steps, std::max<int64_t>(1, (int64_t)tokens * steps / warps));
+  run = (int)std::min<int64_t>(std::min(steps, most), std::max<int64_t>(1, (int64_t)tokens * steps / warps));
   wpt = (steps + run - 1) / run;
   run = (steps + wpt - 1) / wpt;
 }
@@ -231,7 +231,7 @@ extern "C" int lmx_paged_append(const lmx_paged_kv* kv, const lmx_paged_batch* b
   a.ldqo = ldq_out;
   a.err = device_error_word();
   const int steps = (heads + 2 * kv->kv_heads + 512 / D - 1) / (512 / D);
-  warp_runs(batch->tokens, steps, a.run, a.wpt);
+  warp_runs(batch->tokens, steps, kAppendRun, a.run, a.wpt);
   unsigned grid;
   if ((rc = grid_of(((int64_t)batch->tokens * a.wpt + 3) / 4, grid, "paged_append"))) return rc;
   return cuda_check(on_cache(D, kv->bits, [&](auto d, auto bits) {
@@ -250,7 +250,7 @@ extern "C" int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* b
     return set_error(LMX_ERR_INVALID, "paged_gather: k_out and v_out must be 16-byte aligned");
   if (batch->tokens == 0 || batch->seqs == 0 || (!k_out && !v_out)) return LMX_OK;
   GatherArgs a{dev_kv(*kv), dev_batch(*batch), (bf16_t*)k_out, (bf16_t*)v_out, 0, 0, device_error_word()};
-  warp_runs(batch->tokens, (2 * kv->kv_heads * kv->head_dim / 16 + 31) / 32, a.run, a.wpt);
+  warp_runs(batch->tokens, (2 * kv->kv_heads * kv->head_dim / 16 + 31) / 32, 1 << 20, a.run, a.wpt);
   unsigned grid;
   if ((rc = grid_of(((int64_t)batch->tokens * a.wpt + 3) / 4, grid, "paged_gather"))) return rc;
   return cuda_check(on_cache(kv->head_dim, kv->bits, [&](auto d, auto bits) {

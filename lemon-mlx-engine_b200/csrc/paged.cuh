@@ -41,6 +41,34 @@ LMX_DEV uint32_t bf2_fma3(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+// pairs of fp32 in one instruction; each product, sum and difference rounded as by itself
+LMX_DEV uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+LMX_DEV void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+LMX_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+LMX_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+LMX_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+LMX_DEV uint64_t f2_sub(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 LMX_DEV void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -221,13 +249,18 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
 // the rotation above a lane holds 16 values of a head, eight pairs of the
 // rotation or 16 neighbours, so that pairs never cross lanes; the RMSNorm and
 // the quantizer's min / max are shuffles within the head's D / 16 lanes, and the
-// token's sequence, page and cos / sin are looked up once per warp.  The loop over
-// the run is not unrolled (unrolled by four, an earlier form outgrew the
-// instruction cache) but loads two steps ahead, seven CTAs to an SM (4-bit prompts,
-// 7.1k tokens of 80 heads with the rows read back: 79 us with six, 75 with seven, 91 with eight).  The run is as long as leaves the
-// SMs full of warps: long runs share the look-ups, short ones keep a decode
-// step's latency down.  fp32 throughout, rounded once; products and sums of the
-// rotation are rounded separately.
+// token's sequence, page and cos / sin are looked up once per warp, while the run's
+// rows are on their way to shared memory.  The run is as long as leaves the SMs
+// full of warps, four steps at most: long runs share the look-ups, short ones
+// keep a decode step's latency down.  fp32 throughout, rounded once; products and
+// sums of the rotation are rounded separately.
+//
+// Measured: 4.6k tokens of 48 heads with norms into a bf16 cache 26 us (115 MB,
+// 4.4 TB/s); 7.1k tokens of 80 heads into a 4-bit cache, rows read back, 72 us
+// (311 MB, 4.3 TB/s); 32 tokens of 48 64-wide heads 2.7 us.  Half the issue slots
+// are taken and 28 warps per SM resident on average over three waves of short
+// CTAs; register loads two steps ahead took 78 us for the second, runs of six or
+// eight steps 75 to 78, six CTAs an SM 78.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   PagedKv kv;
@@ -244,6 +277,11 @@ struct AppendArgs {
   int run, wpt;          // steps of a warp, warps of a token
   unsigned* err;
 };
+
+static constexpr int kAppendRun = 4;  // steps of a warp at most
+LMX_DEV void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
 
 // codes rint((x - b) / s), clamped to [0, nb].  A product with 1 / s is within
 // 1e-4 of the quotient (which is below 256), so only quotients that close to a
@@ -278,7 +316,7 @@ LMX_DEV void store_codes(uint8_t* dst, const uint32_t (&q)[8]) {
 }
 
 template <int D, int BITS>
-__global__ void __launch_bounds__(128, 7) paged_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(128, 8) paged_append_kernel(AppendArgs a) {
   constexpr int U = D / 16, HPW = 32 / U, NG = D / 64;
   grid_wait();
   grid_launch_dependents();
@@ -293,21 +331,25 @@ __global__ void __launch_bounds__(128, 7) paged_append_kernel(AppendArgs a) {
   const bool turns = a.ct && 16 * u < a.rot, halves = turns && !a.inter;
   const int d0 = halves ? 8 * u : 16 * u, d1 = halves ? a.rot / 2 + 8 * u : d0 + 8;
 
-  auto load = [&](int hh, uint4& v0, uint4& v1) {
+  // The rows do not depend on the token's place: all of the run's are on their
+  // way, each lane's into its own slots, while that is looked up.
+  __shared__ uint4 rows_in[4][kAppendRun][2][32];
+  uint4(*mine)[2][32] = rows_in[threadIdx.x >> 5];
+#pragma unroll 1
+  for (int k = 0; k < a.run; ++k) {
+    const int hh = h + k * HPW;
     if (hh < end) {
       const bf16_t* src = hh < a.heads ? a.q + (int64_t)hh * D
                           : hh < a.heads + a.kv.Hk ? a.k + (int64_t)(hh - a.heads) * D
                                                    : a.v + (int64_t)(hh - a.heads - a.kv.Hk) * D;
       const bool v = hh >= a.heads + a.kv.Hk;  // v heads are not turned: any 16 values do
       src += (int64_t)t * a.ld;
-      v0 = *reinterpret_cast<const uint4*>(src + (v ? 16 * u : d0));
-      v1 = *reinterpret_cast<const uint4*>(src + (v ? 16 * u + 8 : d1));
+      cp_async16(&mine[k][0][lane], src + (v ? 16 * u : d0));
+      cp_async16(&mine[k][1][lane], src + (v ? 16 * u + 8 : d1));
+    } else {
+      mine[k][0][lane] = mine[k][1][lane] = make_uint4(0, 0, 0, 0);
     }
-  };
-  // the rows do not depend on the token's place: load the first before looking it up
-  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0, m0 = n0, m1 = n0;
-  load(h, n0, n1);
-  load(h + HPW, m0, m1);
+  }
   const int seq = paged_seq(a.b, t, lane);
   if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;  // padding
   const int pos = __ldg(a.b.kv_len + seq) - (__ldg(a.b.q_start + seq + 1) - t);
@@ -323,29 +365,35 @@ __global__ void __launch_bounds__(128, 7) paged_append_kernel(AppendArgs a) {
     load8f(a.st + (int64_t)pos * (a.rot / 2) + 8 * u, s);
   }
 
+  asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-  for (; h - sub < end; h += HPW) {  // warp-uniform
+  for (int k = 0; h - sub < end; h += HPW, ++k) {  // warp-uniform
     const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv.Hk, live = h < end;
     float x[16];
-    bf8_unpack(n0, *reinterpret_cast<float(*)[8]>(x));
-    bf8_unpack(n1, *reinterpret_cast<float(*)[8]>(x + 8));
-    n0 = m0;
-    n1 = m1;
-    load(h + 2 * HPW, m0, m1);
+    bf8_unpack(mine[k][0][lane], *reinterpret_cast<float(*)[8]>(x));
+    bf8_unpack(mine[k][1][lane], *reinterpret_cast<float(*)[8]>(x + 8));
     const int e0 = is_q || is_k ? d0 : 16 * u, e1 = is_q || is_k ? d1 : 16 * u + 8;
     if (a.qn) {
-      float p = 0.0f;
+      uint64_t p2 = 0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) p = __fmaf_rn(x[e], x[e], p);
-      p = warp_sum_xor(p, U / 2, 1);
+      for (int e = 0; e < 16; e += 2) {
+        const uint64_t v = f2_pack(x[e], x[e + 1]);
+        p2 = f2_fma(v, v, p2);
+      }
+      float p, odd;
+      f2_unpack(p2, p, odd);
+      p = warp_sum_xor(__fadd_rn(p, odd), U / 2, 1);
       if (is_q || is_k) {
-        const float f = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fmul_rn(p, 1.0f / D), a.eps)));
+        const float f = rsqrtf(__fmaf_rn(p, 1.0f / D, a.eps));  // 2 ulp
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float wn[8];
           bf8_unpack(__ldg(reinterpret_cast<const uint4*>((is_q ? a.qn : a.kn) + (k ? e1 : e0))), wn);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[8 * k + e] = __fmul_rn(__fmul_rn(x[8 * k + e], f), wn[e]);
+          for (int e = 0; e < 8; e += 2) {
+            float* y = x + 8 * k + e;
+            f2_unpack(f2_mul(f2_mul(f2_pack(y[0], y[1]), f2_pack(f, f)), f2_pack(wn[e], wn[e + 1])), y[0], y[1]);
+          }
         }
       }
     }
@@ -359,10 +407,11 @@ __global__ void __launch_bounds__(128, 7) paged_append_kernel(AppendArgs a) {
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float xa = x[e], xb = x[8 + e];
-          x[e] = __fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e]));
-          x[8 + e] = __fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e]));
+        for (int e = 0; e < 8; e += 2) {
+          const uint64_t xa = f2_pack(x[e], x[e + 1]), xb = f2_pack(x[8 + e], x[9 + e]);
+          const uint64_t c2 = f2_pack(c[e], c[e + 1]), s2 = f2_pack(s[e], s[e + 1]);
+          f2_unpack(f2_sub(f2_mul(xa, c2), f2_mul(xb, s2)), x[e], x[e + 1]);
+          f2_unpack(f2_add(f2_mul(xb, c2), f2_mul(xa, s2)), x[8 + e], x[9 + e]);
         }
       }
     }

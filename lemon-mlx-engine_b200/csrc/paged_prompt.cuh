@@ -303,22 +303,6 @@ LMX_DEV void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync
 LMX_DEV void prompt_meet(int tile) { asm volatile("bar.sync %0, 256;" ::"r"(1 + tile) : "memory"); }
 
 // ---- the softmax's pieces, on a thread's row of scores ----
-LMX_DEV uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-LMX_DEV void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-LMX_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-LMX_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 LMX_DEV void prompt_mask(uint32_t* s, int key, int klo, int khi) {
 #pragma unroll
   for (int i = 0; i < 64; ++i)
@@ -517,7 +501,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
   // shared memory, so the dynamic part begins at a multiple of 1024 (checked)
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023) {
-    if (threadIdx.x == 0) atomicExch(p.a.err, 0x51u);
+    if (threadIdx.x == 0) atomicExch(p.a.err, 0x91u);
     return;
   }
   uint8_t* Qs = smem;
@@ -599,7 +583,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       const int klo = row && p.a.window > 0 ? max(0, pos - p.a.window + 1) : 0;
       float m = -INFINITY, l = 0.0f;  // l: this half's
       for (int b = w.b0; b < w.b1; ++b) {
-        ok = ok && prompt_warp_wait(s_full + tile, ps, err, 0x45u);
+        ok = ok && prompt_warp_wait(s_full + tile, ps, err, 0x85u);
         ps ^= 1;
         tmem_fence_after();
         uint32_t s[64];
@@ -642,7 +626,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready + tile);
       }
-      ok = ok && prompt_warp_wait(o_full + tile, po, err, 0x46u);
+      ok = ok && prompt_warp_wait(o_full + tile, po, err, 0x86u);
       // the row's sum from both halves, and once more so that the next item's
       // maxima do not overtake it
       *mine = l;
@@ -733,7 +717,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t(&sb)[IT] = h ? sv : sk;
-            ok = prompt_warp_wait(raw_full + rs, prs, err, 0x54u) && prompt_warp_wait(kv_free + st, pst, err, 0x55u);
+            ok = prompt_warp_wait(raw_full + rs, prs, err, 0x94u) && prompt_warp_wait(kv_free + st, pst, err, 0x95u);
             if (!ok) break;
             const uint8_t* src = raw + rs * SM::RAW + r0 * (D * BITS / 8) + u * (2 * BITS);
             uint8_t* dst = KV + st * TILE;
@@ -758,7 +742,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
               mbar_arrive(raw_free + rs);
             }
             if (h == 0 && b == w.b0) {  // Q comes behind the first tiles
-              ok = prompt_warp_wait(q_raw, pq, err, 0x53u);
+              ok = prompt_warp_wait(q_raw, pq, err, 0x93u);
               if (!ok) break;
               pq ^= 1;
               const int chunks = (w.second(p) ? 2 : 1) * (TILE / 16);
@@ -805,7 +789,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       };
       for (w.begin(p, share); ok && w.live(); w.next(p)) {
         const int tiles = w.second(p) ? 2 : 1, n = w.b1 - w.b0;
-        if (!wait(q_full, pq, 0x47u) || !wait(kv_full + st, pst, 0x48u)) break;
+        if (!wait(q_full, pq, 0x87u) || !wait(kv_full + st, pst, 0x88u)) break;
         pq ^= 1;
         tmem_fence_after();
         if (lead) {
@@ -823,16 +807,16 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
           const bool more = j + 1 < n;
           const int sv = st, sk = st + 1 == NS ? 0 : st + 1;
           const uint32_t pk = st + 1 == NS ? pst ^ 1 : pst;
-          if (!wait(kv_full + sv, pst, 0x48u)) break;
+          if (!wait(kv_full + sv, pst, 0x88u)) break;
           if (BITS == 16 && ((w.z.kb + w.b0 + j + 1) << 7) > w.z.len) {
-            if (!wait(vfix, pfix, 0x49u)) break;
+            if (!wait(vfix, pfix, 0x89u)) break;
             pfix ^= 1;
           }
-          if (more && !wait(kv_full + sk, pk, 0x48u)) break;
+          if (more && !wait(kv_full + sk, pk, 0x88u)) break;
           for (int i = 0; i < tiles; ++i) {
-            if (!wait(p_ready + i, (pp >> i) & 1, 0x4Au)) break;
+            if (!wait(p_ready + i, (pp >> i) & 1, 0x8Au)) break;
             // O of the previous item has been read
-            if (j == 0 && !wait(o_free + i, (pof >> i) & 1, 0x4Bu)) break;
+            if (j == 0 && !wait(o_free + i, (pof >> i) & 1, 0x8Bu)) break;
             tmem_fence_after();
             if (lead) {
               const uint32_t b = (k0 + sv * (TILE >> 4)) | kDescV;
@@ -864,7 +848,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       if (!ok) {  // a wait gave up: let the issued MMAs finish before the memory goes
         if (lead) umma_commit(drain);
         __syncwarp();
-        prompt_wait(drain, 0, err, 0x4Eu);
+        prompt_wait(drain, 0, err, 0x8Eu);
       }
     } else if (warp == kMma + 1) {
       // -------------------------------- loads --------------------------------
@@ -894,7 +878,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
           }
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            ok = prompt_warp_wait(free_ + st, pst, err, 0x4Du);
+            ok = prompt_warp_wait(free_ + st, pst, err, 0x8Du);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)BYTES);
             __syncwarp();
@@ -908,7 +892,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
           if (b == w.b0 && ok) {
             // Q behind the item's first K and V: its memory is free only when the
             // previous item's last scores are done
-            ok = prompt_warp_wait(q_free, pq, err, 0x4Cu);
+            ok = prompt_warp_wait(q_free, pq, err, 0x8Cu);
             if (!ok) break;
             pq ^= 1;
             started = true;
@@ -924,8 +908,8 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
       }
       // leave no copy in flight behind, also where a wait gave up
       for (int k = max(0, issued - N); k < issued; ++k)
-        prompt_wait(full + k % N, (uint32_t)((k / N) & 1), err, 0x4Eu);
-      if (started) prompt_wait(qbar, pq, err, 0x4Eu);
+        prompt_wait(full + k % N, (uint32_t)((k / N) & 1), err, 0x8Eu);
+      if (started) prompt_wait(qbar, pq, err, 0x8Eu);
     } else if (BITS == 16 && warp == kMma + 2) {
       // ------------------ V rows past the sequence's end := 0 ------------------
       int st = 0;
@@ -935,7 +919,7 @@ __global__ void __launch_bounds__(prompt_threads(BITS), 1)
         for (int b = w.b0; b < w.b1 && ok; ++b) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            ok = prompt_warp_wait(kv_full + st, pst, err, 0x4Fu);
+            ok = prompt_warp_wait(kv_full + st, pst, err, 0x8Fu);
             if (!ok) break;
             const int key = (w.z.kb + b) << 7;
             if (kv == 1 && key + 128 > w.z.len) {

@@ -351,7 +351,10 @@ __global__ void __launch_bounds__(128, 8) paged_append_kernel(AppendArgs a) {
     }
   }
   const int seq = paged_seq(a.b, t, lane);
-  if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) return;  // padding
+  if (seq >= a.b.seqs || t < __ldg(a.b.q_start)) {  // padding
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
   const int pos = __ldg(a.b.kv_len + seq) - (__ldg(a.b.q_start + seq + 1) - t);
   int64_t row = -1;
   if (pos >= 0) {

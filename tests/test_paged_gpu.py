@@ -420,6 +420,74 @@ def test_attention_many_sequences(lmx, cuda):
     check(cache, q, got, lse, 0.125, 0)
 
 
+@pytest.mark.parametrize("rows", [0, 1])
+def test_pages_past_four_gigabytes(lmx, cuda, prompt_rows, rows):
+    # K and V interleaved in one pool of 4.7 GB (page_stride), the sequence's pages at its far end
+    prompt_rows(rows)
+    P_, hk, d, pages = 256, 1, 128, 36000
+    pool = torch.zeros(pages * 2 * P_ * d, dtype=BF16, device="cuda")
+    kv = lmx.PagedKvDesc(pages, P_, hk, d, 16, 2 * P_, pool.data_ptr(), pool.data_ptr() + P_ * d * 2)
+    n = 300
+    table = torch.tensor([[pages - 1, pages - 3]], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    batch = lmx.PagedBatch(1, n, n, start.data_ptr(), length.data_ptr(), table.data_ptr(), 2)
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn((n, 4, d), generator=gen).to(BF16).cuda()  # two q heads, k, v
+    q = torch.empty((n, 2, d), dtype=BF16, device="cuda")
+    lmx.call("lmx_paged_append", kv, batch, None, x.data_ptr(), x.data_ptr() + 4 * d, x.data_ptr() + 6 * d, 4 * d, 2, None,
+             None, 0.0, q.data_ptr(), 2 * d, None)
+    back = [torch.empty((n, 1, d), dtype=BF16, device="cuda") for _ in "kv"]
+    lmx.call("lmx_paged_gather", kv, batch, back[0].data_ptr(), back[1].data_ptr(), None)
+    assert torch.equal(q, x[:, :2]) and torch.equal(back[0], x[:, 2:3]) and torch.equal(back[1], x[:, 3:])
+    at = (pages - 1) * 2 * P_ * d
+    assert torch.equal(pool[at:at + P_ * d].view(P_, d), x[:P_, 2]) and torch.equal(pool[at + P_ * d:].view(P_, d), x[:P_, 3])
+    size = lmx.lib().lmx_paged_attention_scratch_bytes(kv, batch, 2)
+    scratch, out = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty_like(q)
+    lmx.call("lmx_paged_attention", kv, batch, q.data_ptr(), 2 * d, 2, 0.09, 0, scratch.data_ptr(), size, out.data_ptr(),
+             2 * d, None, None)
+    z = torch.einsum("qhd,kd->hqk", x[:, :2].double(), x[:, 2].double()) * 0.09
+    z.masked_fill_(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    p = torch.softmax(z, -1)
+    want = torch.einsum("hqk,kd->qhd", p, x[:, 3].double())
+    A = torch.einsum("hqk,kd->qhd", p, x[:, 3].double().abs())
+    # bf16 output; p as bf16 in the prompt kernel; scores to 128 2^-24 of their terms' sum (below 2^5 here)
+    assert ((out.double() - want).abs() <= U * want.abs() + A * (2.0 ** -8 + 2.0 ** -11)).all()
+
+
+def test_calls_in_a_cuda_graph(lmx, cuda):
+    cache = P.Cache(17, [(1, 200), (70, 300), (1, 33)], 2, 128, 8, 32)
+    kv, batch = cache.device(lmx)
+    n = cache.tokens
+    c, s = table(lmx, 0, 512, 128)
+    x = torch.randn((n, 12 * 128), generator=cache.gen).to(BF16).cuda()
+    q, out = (torch.empty((n, 8 * 128), dtype=BF16, device="cuda") for _ in "qo")
+    size = lmx.lib().lmx_paged_attention_scratch_bytes(kv, batch, 8)
+    scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+    def step(stream):
+        lmx.call("lmx_paged_append", kv, batch, desc(lmx, c, s, 0), x.data_ptr(), x.data_ptr() + 2048, x.data_ptr() + 2560,
+                 12 * 128, 8, None, None, 0.0, q.data_ptr(), 1024, stream)
+        lmx.call("lmx_paged_attention", kv, batch, q.data_ptr(), 1024, 8, 0.088, 0, scratch.data_ptr(), size, out.data_ptr(),
+                 1024, None, stream)
+
+    step(None)
+    torch.cuda.synchronize()
+    first = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(torch.cuda.current_stream().cuda_stream)
+    # the lengths are read on the device: the same graph serves other ones
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+    cache.index[1][2] = 20
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[:71], first[:71]) and not torch.equal(out[71], first[71])
+
+
 def test_attention_missing_page_reads_zeros(lmx, cuda):
     cache = P.Cache(15, [(1, 50)], 1, 64, 16, 16)
     cache.table[0, 1] = cache.pages + 5

@@ -162,6 +162,8 @@ LMX_DEV void load8f(const float* p, float (&x)[8]) {
 // a token -- 8 pairs (two 16-byte halves, rot/2 apart, or 16 neighbours when
 // interleaved), so both layouts move whole 16-byte vectors and the unit's
 // cos / sin stay in registers over the heads; units past rot are copied.
+// Measured: 8191 tokens of 40 128-wide heads 28.9 us (170 MB, 5.9 TB/s: 90 % of
+// the copy rate); 8 tokens of 24 heads 2.6 us.
 // ---------------------------------------------------------------------------
 struct RopeArgs {
   const float *ct, *st;
@@ -485,7 +487,8 @@ __global__ void __launch_bounds__(128, 8) paged_append_kernel(AppendArgs a) {
 // ---------------------------------------------------------------------------
 // Gather: the batch's rows back as bf16(fma(scale, code, bias)).  A lane owns
 // 16 values of a token's K heads, then V heads, at a time; a warp `run` times 32
-// such units of one token.
+// such units of one token.  Memory bound; 80 tokens of 8 heads take 4 us, the
+// latency of the look-ups.
 // ---------------------------------------------------------------------------
 struct GatherArgs {
   PagedKv kv;
@@ -585,6 +588,12 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(GatherArgs a) {
 //   sum_j p_j v_j = sum_j (p_j s_j) (c_j - z) + sum_j p_j (b_j + z s_j),
 // z = 8 or 128 being the middle of the code range, so that the first sum
 // does not cancel against the second.
+//
+// Measured, one token of 16 sequences over up to 8000 rows, 8 KV heads of 128:
+// bf16 pages 74 us (5.9 TB/s, 90 % of the copy rate), 8-bit 63 us (3.5 TB/s), 4-bit
+// 61 us; the last two are bound by the 430 to 440 instructions a warp spends on
+// 16 keys, most of them unpacking codes.  One sequence of 700 rows: 8 us with the
+// join, the latency of six dependent look-ups and two launches.
 // ---------------------------------------------------------------------------
 // Shape of the few-row kernel.  KP: 16-key groups that a warp takes at a time;
 // two share a maximum, a rescale and the index work (64-wide 4-bit heads, 16 x

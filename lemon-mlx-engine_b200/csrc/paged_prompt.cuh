@@ -4,19 +4,23 @@
 // The G query heads of a KV head times TT = 128 / G tokens are one 128-row
 // tile (row t*G + g), so grouped heads share every K and V tile; an item is
 // (sequence, KV head, pair of row tiles), and its keys go in tiles of 128:
-//   S = Q K^T         (128 x 128 x D, both operands in shared memory)
-//   p = 2^(s - m), l += sum p        (one thread per row)
-//   O += P V          (128 x D x 128, P in tensor memory)
+//   S = Q K^T                        (128 x 128 x D, both operands in shared memory)
+//   p = 2^(s - m), l += sum p        (two threads per row)
+//   O += P V                         (128 x D x 128, P in tensor memory)
 // For D = 128 a key tile of one row tile costs 1024 tensor cycles and 128 * 128
 // exponentials, 1024 cycles of the SM's special-function unit: the two row
 // tiles of a pair take turns, one in the tensor pipe while the other is in
-// its softmax, so both units stay busy.
+// its softmax.
 //
 // Warps: 0-7 and 8-15 softmax and epilogue of the pair's first and second tile
-// (two threads per row, one for each half of the keys and of the head dims);
+// (two threads per row, one for each half of the keys and of the head dims: one
+// thread per row left the schedulers two warps each, too few to hide latency);
 // 16 issues the MMAs; 17 loads (TMA: one box per page and 64 head dims, so the
-// tile in shared memory is the same whatever the page size); 18 follows the loads and clears the V rows of a tile that lie past the
-// sequence's end (p = 0 there, but 0 * NaN is not 0).
+// tile in shared memory is the same whatever the page size); 18 follows the
+// loads and clears the V rows of a tile that lie past the sequence's end (p = 0
+// there, but 0 * NaN is not 0).  Quantized caches: 17 loads packed tiles, and
+// warps 20-27 turn them into fp16 K and V tiles, zero rows included.
+//
 // Tensor memory: S of the two tiles [0, 256), O at 256; P (16-bit) overlays
 // the first half of its S, which the softmax has then read.  MMAs issued by
 // one thread run in order, so "S(j+1) done" also says that P(j) has been used
@@ -28,9 +32,16 @@
 //
 // Work split: as in the few-row kernel, the 128-key blocks of all items are
 // laid end to end, each item with a fixed cost of its own in front, and divided
-// evenly over one CTA per SM; items that cross a
-// boundary leave fp32 partials that paged_prompt_join_kernel adds in order.
-// Every CTA works the division out for itself (prompt_plan).
+// evenly over one CTA per SM; items that cross a boundary leave fp32 partials
+// that paged_prompt_join_kernel adds in order.  Every CTA works the division out
+// for itself (prompt_plan).
+//
+// Measured: one 8192-token prompt of 64 / 8 heads of 128 0.94 to 0.98 ms (1.13 to
+// 1.17 PFLOP/s of visible pairs; back to back, at the power limit, 1.06 ms), 2048
+// tokens 93 us, over 8-bit pages 116 us, 4-bit 127 us; ragged prompts to 4000
+// tokens of 32 / 8 heads of 64 203 us.  Bound by a row tile's chain of scores,
+// softmax and P V: 56 % of the tensor pipe is busy, 42 % of the special-function
+// unit (D = 128).
 #pragma once
 #include "paged.cuh"
 #include "sm100.cuh"

@@ -38,7 +38,7 @@
 //
 // Measured: one 8192-token prompt of 64 / 8 heads of 128 0.94 to 0.98 ms (1.13 to
 // 1.17 PFLOP/s of visible pairs; back to back, at the power limit, 1.06 ms), 2048
-// tokens 93 us, over 8-bit pages 116 us, 4-bit 127 us; ragged prompts to 4000
+// tokens 92 us, over 8-bit pages 112 us, 4-bit 121 us; ragged prompts to 4000
 // tokens of 32 / 8 heads of 64 203 us.  Bound by a row tile's chain of scores,
 // softmax and P V: 56 % of the tensor pipe is busy, 42 % of the special-function
 // unit (D = 128).
@@ -359,11 +359,15 @@ LMX_DEV void ex2_pair(uint64_t x, float& p0, float& p1) {
   p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
   p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
 }
-// p = 2^(s * scale2 + ms) of 64 scores, stored as pairs (bf16; fp16
-// for quantized caches); returns their sum.  Of eight pairs kPromptFma go to the FMA pipe: the special-function unit
-// alone would take as long as the MMAs (D = 128) or twice that (D = 64; ragged
-// 64-wide prompts 268 us with 0, 248 with 2, 278 with 4; D = 128 the same with 0 and 2).
-static constexpr int kPromptFma = 2;
+// Of eight pairs of exponentials kPromptFma go to the FMA pipe: the special-
+// function unit alone would take as long as the MMAs (D = 128) or twice that (D =
+// 64; ragged 64-wide prompts 221 us with 0, 216 with 1, 203 with 2; D = 128 alike).
+// Over quantized caches the dequantizing warps want the issue slots (2048 tokens
+// of 64 128-wide heads, 8 bits: 112 us with 0, 116 with 2; 4 bits 121 and 126).
+template <int BITS>
+static constexpr int kPromptFma = BITS == 16 ? 2 : 0;
+// p = 2^(s * scale2 + ms) of 64 scores, stored as pairs (bf16; fp16 for quantized
+// caches); returns their sum.
 template <int BITS>
 LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP) {
   const uint64_t sc = f2_pack(scale2, scale2), mm = f2_pack(ms, ms);
@@ -375,7 +379,7 @@ LMX_DEV float prompt_exp(const uint32_t* s, float scale2, float ms, uint32_t tP)
     for (int i = 0; i < 16; ++i) {
       const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[32 * h + 2 * i]), __uint_as_float(s[32 * h + 2 * i + 1])), sc, mm);
       float p0, p1;
-      if (i % 8 >= 8 - kPromptFma) {
+      if (i % 8 >= 8 - kPromptFma<BITS>) {
         ex2_pair(x, p0, p1);
       } else {
         f2_unpack(x, p0, p1);

@@ -333,9 +333,10 @@ int lmx_paged_gather(const lmx_paged_kv* kv, const lmx_paged_batch* batch, void*
  * q, out [tokens][heads][head_dim] bf16, token rows ldq / ldo values apart
  * (out must not overlap q); lse fp32 [tokens][heads] or NULL.  heads is a
  * multiple of kv_heads, at most 64 times it.  A row that sees nothing gives
- * zeros and lse -infinity.  Rows of a page that no sequence
- * position covers may hold anything (NaN included); every row below kv_len
- * must hold finite values.  scratch: lmx_paged_attention_scratch_bytes of the
+ * zeros and lse -infinity.  Rows at or past kv_len may hold
+ * anything (NaN included), and a table entry whose page lies wholly before
+ * every new token's window is not used; the rows of the other pages below
+ * kv_len must hold finite values.  scratch: lmx_paged_attention_scratch_bytes of the
  * same kv / batch / heads (0 and a message in lmx_last_error when the
  * arguments are refused), 16-byte aligned, contents arbitrary; calls that
  * overlap need scratch of their own.  Waits inside the prompt kernel are

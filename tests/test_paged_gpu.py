@@ -488,6 +488,49 @@ def test_calls_in_a_cuda_graph(lmx, cuda):
     assert torch.equal(out[:71], first[:71]) and not torch.equal(out[71], first[71])
 
 
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("rows", [0, 1])
+def test_pages_before_the_window_may_be_gone(lmx, cuda, prompt_rows, bits, rows):
+    # rows that no query sees any more: their table entries name nothing, or a page of NaN
+    prompt_rows(rows)
+    lens, window = [(3, 300), (70, 500), (1, 20)], 50
+    cache = P.Cache(18, lens, 2, 128, bits, 16, spare=0)
+    for i, (new, n) in enumerate(lens):
+        gone = max(0, n - new - window + 1) // 16
+        cache.table[i, :gone] = -1
+        cache.table[i, :gone:2] = cache.pages - 1 if cache.pages - 1 not in cache.table[i] else -1
+    q = torch.randn((cache.tokens, 6, 128), generator=cache.gen).to(BF16)
+    P.device_error(lmx)
+    got, lse = attend(lmx, cache, q, 6, 0.09, window)
+    assert P.device_error(lmx) == 0
+    if rows == 0:
+        check(cache, q, got, lse, 0.09, window)
+    elif bits == 16:
+        check(cache, q, got, lse, 0.09, window, p_err=2.0 ** -8)
+    else:
+        check(cache, q, got, lse, 0.09, window, p_err=2.0 ** -11, kv_err=2.0 ** -11)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_prompt_kernel_unaligned_output_and_far_stride(lmx, cuda, prompt_rows, bits):
+    # outputs 16- but not 32-byte aligned take the narrow stores
+    prompt_rows(1)
+    cache = P.Cache(19, [(100, 250), (1, 3)], 1, 64, bits, 64)
+    kv, batch = cache.device(lmx)
+    q = torch.randn((101, 4, 64), generator=cache.gen).to(BF16)
+    dq = q.cuda()
+    size = lmx.lib().lmx_paged_attention_scratch_bytes(kv, batch, 4)
+    scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+    res = []
+    for off, ld in ((0, 256), (8, 264)):
+        out = torch.full((102 * 264,), 9.0, dtype=BF16, device="cuda")
+        lmx.call("lmx_paged_attention", kv, batch, dq.data_ptr(), 256, 4, 0.125, 0, scratch.data_ptr(), size,
+                 out.data_ptr() + 2 * off, ld, None, None)
+        res.append(out[off:off + 101 * ld].view(101, ld)[:, :256].clone())
+        assert (out[:off] == 9.0).all() and (out[off + 101 * ld:] == 9.0).all()
+    assert torch.equal(res[0], res[1])
+
+
 def test_attention_missing_page_reads_zeros(lmx, cuda):
     cache = P.Cache(15, [(1, 50)], 1, 64, 16, 16)
     cache.table[0, 1] = cache.pages + 5

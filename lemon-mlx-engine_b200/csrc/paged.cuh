@@ -41,7 +41,7 @@ LMX_DEV uint32_t bf2_fma3(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-// pairs of fp32 in one instruction; each product, sum and difference rounded as by itself
+// pairs of fp32 in one instruction
 LMX_DEV uint64_t f2_pack(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -58,14 +58,14 @@ LMX_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-LMX_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 LMX_DEV uint64_t f2_sub(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+LMX_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 
@@ -257,9 +257,9 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
 // keep a decode step's latency down.  fp32 throughout, rounded once; products and
 // sums of the rotation are rounded separately.
 //
-// Measured: 4.6k tokens of 48 heads with norms into a bf16 cache 26 us (115 MB,
-// 4.4 TB/s); 7.1k tokens of 80 heads into a 4-bit cache, rows read back, 72 us
-// (311 MB, 4.3 TB/s); 32 tokens of 48 64-wide heads 2.7 us.  Half the issue slots
+// Measured: 4.6k tokens of 48 heads with norms into a bf16 cache 27 us (115 MB,
+// 4.3 TB/s); 7.1k tokens of 80 heads into a 4-bit cache, rows read back, 75 us
+// (311 MB, 4.2 TB/s); 32 tokens of 48 64-wide heads 2.7 us.  Half the issue slots
 // are taken and 28 warps per SM resident on average over three waves of short
 // CTAs; register loads two steps ahead took 78 us for the second, runs of six or
 // eight steps 75 to 78, six CTAs an SM 78.
@@ -330,6 +330,8 @@ __global__ void __launch_bounds__(128, 8) paged_append_kernel(AppendArgs a) {
   int h = (int)(w % a.wpt) * a.run * HPW + sub;  // this lane's head; the warp's steps are HPW apart
   const int end = min(nh, h - sub + a.run * HPW);
   // this lane's two runs of eight values
+  const float no = __int_as_float(a.heads >> 31);  // 0
+  const uint64_t zero = f2_pack(no, no);
   const bool turns = a.ct && 16 * u < a.rot, halves = turns && !a.inter;
   const int d0 = halves ? 8 * u : 16 * u, d1 = halves ? a.rot / 2 + 8 * u : d0 + 8;
 
@@ -411,12 +413,14 @@ __global__ void __launch_bounds__(128, 8) paged_append_kernel(AppendArgs a) {
           x[2 * e + 1] = __fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e]));
         }
       } else {
+        // Products as fma(., ., 0) with a zero that the compiler does not know: it
+        // fuses a paired product and sum, and a rounding less may make another code.
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const uint64_t xa = f2_pack(x[e], x[e + 1]), xb = f2_pack(x[8 + e], x[9 + e]);
           const uint64_t c2 = f2_pack(c[e], c[e + 1]), s2 = f2_pack(s[e], s[e + 1]);
-          f2_unpack(f2_sub(f2_mul(xa, c2), f2_mul(xb, s2)), x[e], x[e + 1]);
-          f2_unpack(f2_add(f2_mul(xb, c2), f2_mul(xa, s2)), x[8 + e], x[9 + e]);
+          f2_unpack(f2_sub(f2_fma(xa, c2, zero), f2_fma(xb, s2, zero)), x[e], x[e + 1]);
+          f2_unpack(f2_add(f2_fma(xb, c2, zero), f2_fma(xa, s2, zero)), x[8 + e], x[9 + e]);
         }
       }
     }

@@ -217,6 +217,32 @@ def test_append_and_gather(lmx, cuda, bits, lens, hk, g, d, page, rot, inter, no
     assert (got_q[cache.start[-1]:] == 9.0).all() and (ko[cache.start[-1]:] == 9.0).all()
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("inter", [0, 1])
+@pytest.mark.parametrize("rot", [64, 128])
+def test_rotated_codes_are_those_of_fp32(lmx, cuda, bits, inter, rot):
+    # every product, sum and quotient of the rule rounded by itself in fp32: the codes come out the same
+    cache = P.Cache(4, [(500, 700)], 4, 128, bits, 32)
+    kv, batch = cache.device(lmx)
+    c, s = table(lmx, 0, 1024, rot)
+    x = torch.randn((500, 8 * 128), generator=cache.gen).to(BF16)
+    dx = x.cuda()
+    lmx.call("lmx_paged_append", kv, batch, desc(lmx, c, s, inter), None, dx.data_ptr(), dx.data_ptr() + 1024, 1024, 0, None,
+             None, 0.0, None, 0, None)
+    cc, ss = c.cpu()[200:700, None], s.cpu()[200:700, None]
+    k = x[:, :512].reshape(500, 4, 128).float()
+    ia = torch.arange(0, rot, 2) if inter else torch.arange(rot // 2)
+    ib = ia + (1 if inter else rot // 2)
+    y = k.clone()
+    y[..., ia] = k[..., ia] * cc - k[..., ib] * ss
+    y[..., ib] = k[..., ib] * cc + k[..., ia] * ss
+    at = cache.at(0, torch.arange(200, 700))
+    for m, v in (("k", y), ("v", x[:, 512:].reshape(500, 4, 128).float())):
+        q, sc, bi = P.quantize(v, bits)
+        assert torch.equal(cache.dev[m].cpu()[at], P.pack(q, bits))
+        assert torch.equal(cache.dev[m + "s"].cpu()[at], sc) and torch.equal(cache.dev[m + "b"].cpu()[at], bi)
+
+
 def test_append_in_place_and_without_queries(lmx, cuda):
     cache = P.Cache(5, [(3, 9), (2, 2)], 2, 128, 16, 16)
     kv, batch = cache.device(lmx)
